@@ -116,6 +116,7 @@ int lnn_conv2d_fwd_f32(int dev, const lnn_conv2d_desc* d, const float* X, const 
  * which gives bit-identical results to the three separate kernels. */
 #define LNN_ACT_NONE 0
 #define LNN_ACT_LEAKY_RELU 1
+#define LNN_ACT_SILU 2 /* x / (1 + exp(-x)); group normalisation only */
 int lnn_conv2d_fwd_bias_act_f32(int dev, const lnn_conv2d_desc* d, const float* X, const float* W,
                                 const float* bias, int act, float slope, float* Y);
 /* Backward of that epilogue in one pass over y and dy, both [N][O][HW] (the layer's bias add is
@@ -315,6 +316,47 @@ int lnn_adam_update_multi_lrd_f32(int dev, int count, const uint64_t* n, float* 
  * He / Glorot initialisers are these two with derived bounds (initializer/He.py:18-33, Glorot.py:20-35). */
 int lnn_random_uniform_f32(int dev, float* out, uint64_t n, uint32_t seed, double low, double high);
 int lnn_random_normal_f32(int dev, float* out, uint64_t n, uint32_t seed, double mean, double stddev);
+
+/* ---- group normalisation with an activation (no counterpart in the reference, whose normalisation layer is a
+ *      BatchNorm built from separate ops).  x, y, dy, dx are [N][C][HW], or [N][HW][C] with channels_last; a dense
+ *      layer's rows (rows, C) are N = rows, HW = 1.  The C / groups * HW elements of image n whose channel lies in
+ *      group g form row n * groups + g:
+ *        xh = (x - mean[row]) * rstd[row];   y = act(gamma[c] * xh + beta[c])
+ *        rstd = 1 / sqrt(var + eps), var the mean squared distance from the mean
+ *      act: LNN_ACT_NONE, LNN_ACT_LEAKY_RELU with any slope (0: ReLU; the derivative at 0 is 1, as lnn_ew_bwd_f32's),
+ *      LNN_ACT_SILU.  gamma / beta: C values, or NULL for ones / zeros.  eps > 0. */
+typedef struct lnn_group_norm_desc {
+  int32_t N, C, HW, groups;
+  int32_t channels_last, act;
+  float slope, eps;
+} lnn_group_norm_desc;
+/* y, and mean / rstd (N * groups values each) for the backward pass.  x8: NULL, or where to write x in 8 bits
+ * (lnn_encode8_f32's result on x).  The outputs must not overlap x or each other. */
+int lnn_group_norm_fwd_f32(int dev, const lnn_group_norm_desc* d, const float* x, const float* gamma,
+                           const float* beta, float* y, float* mean, float* rstd, void* x8);
+/* dx (+)=, dgamma[c] (+)=, dbeta[c] (+)= the gradients of sum(dy * y), each NULL if not wanted and each with its own
+ * beta.  Exactly one of x (the forward pass's input) and x8 (its 8-bit copy, whose values then stand in for x; mean and
+ * rstd stay the forward pass's) is given.  The outputs must not overlap the inputs or each other.  Sums are added in a
+ * fixed order: the same inputs give the same bits. */
+int lnn_group_norm_bwd_f32(int dev, const lnn_group_norm_desc* d, const float* x, const void* x8, const float* gamma,
+                           const float* beta, const float* mean, const float* rstd, const float* dy,
+                           float* dx, int beta_dx, float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta);
+
+/* ---- activations kept in 8 bits between the forward and the backward pass.
+ *      Every 32 elements that follow each other in memory share a power of two 2^e: with a the largest magnitude among
+ *      them, e is the smallest whole number for which a * 2^-e < 127.5, kept within [-126, 121] (e of a power-of-two range:
+ *      64 <= a * 2^-e < 127.5 wherever neither limit acts).  Codes are round-half-even(x * 2^-e) as int8, within +-127; an
+ *      element reads back as code * 2^e, off by at most half of 2^e.  A copy of n elements is ceil(n / 32) * 32 codes (the
+ *      last block padded with zeros) followed by ceil(n / 32) exponent bytes: e + 127, or 0 for a block of zeros, or 255
+ *      for a block that holds an infinity or a NaN, all of which reads back as NaN. */
+/* bytes of the copy of n elements (host arithmetic) */
+int lnn_bytes8(uint64_t n, uint64_t* bytes);
+int lnn_encode8_f32(int dev, uint64_t n, const float* src, void* dst);
+int lnn_decode8_f32(int dev, uint64_t n, const void* src, float* dst);
+/* Weight gradient of a dense layer from its kept input (matmul.py:64-67, whose first operand is then the 8-bit copy):
+ *   dW[b][k][m] (+)= sum over the rows of X[b][row][k] * dO[b][row][m]
+ * x8 is the copy of the whole dense X [batch][rows][K]; dO [batch][rows][M] and dW [batch][K][M] are dense fp32. */
+int lnn_gemm_wgrad8_f32(int dev, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta);
 
 #ifdef __cplusplus
 }

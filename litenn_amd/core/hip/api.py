@@ -38,6 +38,11 @@ class ConvDesc(ctypes.Structure):
                 ('N', 'C', 'IH', 'IW', 'O', 'KH', 'KW', 'OH', 'OW', 'PADL', 'PADT', 'stride', 'dilation')]
 
 
+class GroupNormDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ('N', 'C', 'HW', 'groups', 'channels_last', 'act')] +
+                [(n, ctypes.c_float) for n in ('slope', 'eps')])
+
+
 _c_int, _c_u32, _c_u64, _c_i64, _c_f32 = ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int64, ctypes.c_float
 _c_f64 = ctypes.c_double
 _ptr = ctypes.c_void_p
@@ -97,6 +102,12 @@ SIGNATURES = {
     'lnn_sgd_update_multi_lrd_f32': [_c_int, _c_int, _ptr, _ptr, _ptr, _ptr, _c_f32, _c_f32, _c_int, _c_f32, _ptr, _ptr, _ptr, _ptr, _ptr],
     'lnn_adam_update_multi_lrd_f32': [_c_int, _c_int, _ptr, _ptr, _ptr, _ptr, _ptr, _c_f32, _c_f32, _c_f32, _c_f32, _ptr, _ptr, _ptr, _ptr, _ptr],
     'lnn_bias_act_bwd_f32': [_c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _c_f32, _ptr, _ptr, _c_int],
+    'lnn_group_norm_fwd_f32': [_c_int, ctypes.POINTER(GroupNormDesc)] + [_ptr] * 7,
+    'lnn_group_norm_bwd_f32': [_c_int, ctypes.POINTER(GroupNormDesc)] + [_ptr] * 8 + [_c_int, _ptr, _c_int, _ptr, _c_int],
+    'lnn_bytes8': [_c_u64, ctypes.POINTER(_c_u64)],
+    'lnn_encode8_f32': [_c_int, _c_u64, _ptr, _ptr],
+    'lnn_decode8_f32': [_c_int, _c_u64, _ptr, _ptr],
+    'lnn_gemm_wgrad8_f32': [_c_int] * 5 + [_ptr] * 3 + [_c_int],
     'lnn_random_uniform_f32': [_c_int, _ptr, _c_u64, _c_u32, _c_f64, _c_f64],
     'lnn_random_normal_f32': [_c_int, _ptr, _c_u64, _c_u32, _c_f64, _c_f64],
 }
@@ -231,7 +242,7 @@ def conv2d_fwd(dev, desc, X, W, Y, beta=0):
     check(lib.lnn_conv2d_fwd_f32(dev, ctypes.byref(desc), X, W, Y, int(beta)))
 
 
-ACT_NONE, ACT_LEAKY_RELU = 0, 1
+ACT_NONE, ACT_LEAKY_RELU, ACT_SILU = 0, 1, 2     # ACT_SILU: group_norm only
 
 
 def conv2d_fwd_bias_act(dev, desc, X, W, bias, act, slope, Y):
@@ -381,6 +392,42 @@ def random_normal(dev, out, n, seed, mean, stddev):
 
 def bias_act_bwd(dev, N, O, HW, y, dy, act, slope, dpre, dbias, beta_bias):
     check(lib.lnn_bias_act_bwd_f32(dev, N, O, HW, y, dy, act, float(slope), dpre, dbias, beta_bias))
+
+
+def group_norm_desc(N, C, HW, groups, channels_last=False, act=ACT_NONE, slope=0.0, eps=1e-5):
+    """Group normalisation of [N][C][HW] (or [N][HW][C]) followed by act (ACT_NONE / ACT_LEAKY_RELU / ACT_SILU)."""
+    return GroupNormDesc(N, C, HW, groups, 1 if channels_last else 0, act, slope, eps)
+
+
+def group_norm_fwd(dev, desc, x, gamma, beta, y, mean, rstd, x8=None):
+    """y, and mean / rstd (N * groups values each); gamma / beta may be None; x8: where to leave x in 8 bits."""
+    check(lib.lnn_group_norm_fwd_f32(dev, ctypes.byref(desc), x, gamma, beta, y, mean, rstd, x8))
+
+
+def group_norm_bwd(dev, desc, x, x8, gamma, beta, mean, rstd, dy, dx, dgamma, dbeta, beta_dx=0, beta_dgamma=0, beta_dbeta=0):
+    """Gradients of group_norm_fwd; x or its 8-bit copy x8 is given, the other is None.  dx, dgamma, dbeta may be None."""
+    check(lib.lnn_group_norm_bwd_f32(dev, ctypes.byref(desc), x, x8, gamma, beta, mean, rstd, dy, dx, int(beta_dx),
+                                     dgamma, int(beta_dgamma), dbeta, int(beta_dbeta)))
+
+
+def bytes8(n):
+    """Bytes of the 8-bit copy of n elements (host arithmetic, needs no device)."""
+    b = _c_u64(0)
+    check(lib.lnn_bytes8(int(n), ctypes.byref(b)))
+    return b.value
+
+
+def encode8(dev, n, src, dst):
+    check(lib.lnn_encode8_f32(dev, int(n), src, dst))
+
+
+def decode8(dev, n, src, dst):
+    check(lib.lnn_decode8_f32(dev, int(n), src, dst))
+
+
+def gemm_wgrad8(dev, batch, rows, K, M, x8, dO, dW, beta=0):
+    """dW[b] (+)= X[b]^T . dO[b] with X [batch][rows][K] in 8 bits, dO [batch][rows][M], dW [batch][K][M]."""
+    check(lib.lnn_gemm_wgrad8_f32(dev, batch, rows, K, M, x8, dO, dW, int(beta)))
 
 
 def _ptr_array(ptrs):

@@ -23,6 +23,12 @@ int launch_update_multi(DeviceCtx*, int, int, const uint64_t*, float* const*, co
                         const uint32_t* = nullptr);
 int launch_bias_act_bwd(DeviceCtx*, int, int, int, const float*, const float*, int, float, float*, float*, int);
 int launch_random_normal(DeviceCtx*, float*, uint64_t, uint32_t, double, double);
+int launch_group_norm_fwd(DeviceCtx*, const lnn_group_norm_desc*, const float*, const float*, const float*, float*, float*, float*, void*);
+int launch_group_norm_bwd(DeviceCtx*, const lnn_group_norm_desc*, const float*, const void*, const float*, const float*, const float*,
+                          const float*, const float*, float*, int, float*, int, float*, int);
+int launch_encode8(DeviceCtx*, uint64_t, const float*, void*);
+int launch_decode8(DeviceCtx*, uint64_t, const void*, float*);
+int launch_wgrad8(DeviceCtx*, int, int, int, int, const void*, const float*, float*, int);
 
 // Scratch of the allocation-free entry point (lnn_conv2d_wgrad_noalloc_f32): split-K partial sums and, for
 // geometries that need one, the gather table.  Every GPU the library runs on holds its own copy of this array
@@ -539,6 +545,53 @@ int lnn_bias_act_bwd_f32(int dev, int N, int O, int HW, const float* y, const fl
                          float* dpre, float* dbias, int beta_bias) {
   CTX(dev);
   return launch_bias_act_bwd(ctx, N, O, HW, y, dy, act, slope, dpre, dbias, beta_bias);
+}
+
+int lnn_group_norm_fwd_f32(int dev, const lnn_group_norm_desc* d, const float* x, const float* gamma, const float* beta, float* y,
+                           float* mean, float* rstd, void* x8) {
+  if (!x || !y || !mean || !rstd) return set_error(LNN_ERR_INVALID, "group_norm_fwd: null pointer");
+  CTX(dev);
+  return launch_group_norm_fwd(ctx, d, x, gamma, beta, y, mean, rstd, x8);
+}
+
+int lnn_group_norm_bwd_f32(int dev, const lnn_group_norm_desc* d, const float* x, const void* x8, const float* gamma,
+                           const float* beta, const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx,
+                           float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta) {
+  if ((x == nullptr) == (x8 == nullptr)) return set_error(LNN_ERR_INVALID, "group_norm_bwd: exactly one of x and x8 must be given");
+  if (!mean || !rstd || !dy) return set_error(LNN_ERR_INVALID, "group_norm_bwd: null pointer");
+  CTX(dev);
+  return launch_group_norm_bwd(ctx, d, x, x8, gamma, beta, mean, rstd, dy, dx, beta_dx, dgamma, beta_dgamma, dbeta, beta_dbeta);
+}
+
+int lnn_bytes8(uint64_t n, uint64_t* bytes) {
+  if (!bytes) return set_error(LNN_ERR_INVALID, "bytes8: null pointer");
+  if (n > kMaxTensorBytes / 4) return set_error(LNN_ERR_UNSUPPORTED, "bytes8: tensor of 2 GiB or more");
+  *bytes = (n + 31) / 32 * 33;
+  return LNN_OK;
+}
+
+int lnn_encode8_f32(int dev, uint64_t n, const float* src, void* dst) {
+  if (n && (!src || !dst)) return set_error(LNN_ERR_INVALID, "encode8: null pointer");
+  if (n > kMaxTensorBytes / 4) return set_error(LNN_ERR_UNSUPPORTED, "encode8: tensor of 2 GiB or more");
+  CTX(dev);
+  return n ? launch_encode8(ctx, n, src, dst) : LNN_OK;
+}
+
+int lnn_decode8_f32(int dev, uint64_t n, const void* src, float* dst) {
+  if (n && (!src || !dst)) return set_error(LNN_ERR_INVALID, "decode8: null pointer");
+  if (n > kMaxTensorBytes / 4) return set_error(LNN_ERR_UNSUPPORTED, "decode8: tensor of 2 GiB or more");
+  CTX(dev);
+  return n ? launch_decode8(ctx, n, src, dst) : LNN_OK;
+}
+
+int lnn_gemm_wgrad8_f32(int dev, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta) {
+  if (batch < 1 || rows < 1 || K < 1 || M < 1) return set_error(LNN_ERR_INVALID, "gemm_wgrad8: extents must be >= 1");
+  if (!x8 || !dO || !dW) return set_error(LNN_ERR_INVALID, "gemm_wgrad8: null pointer");
+  const uint64_t most = kMaxTensorBytes / 4, br = (uint64_t)batch * rows;
+  if (br > most || (uint64_t)batch * K > most || br * K > most || br * M > most || (uint64_t)batch * K * M > most)
+    return set_error(LNN_ERR_UNSUPPORTED, "gemm_wgrad8: tensor of 2 GiB or more");
+  CTX(dev);
+  return launch_wgrad8(ctx, batch, rows, K, M, x8, dO, dW, beta);
 }
 
 int lnn_random_uniform_f32(int dev, float* out, uint64_t n, uint32_t seed, double low, double high) {
