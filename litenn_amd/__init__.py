@@ -31,6 +31,8 @@ from litenn_amd.core.op.depthwise_conv2D import depthwise_conv2D
 from litenn_amd.core.op.dual_wise_op import add, sub, mul
 from litenn_amd.core.op.element_wise_op import (add_const, sub_const, mul_const, div_const,
                                                 leaky_relu, relu, square)
+from litenn_amd.core.op.group_norm import group_norm
+from litenn_amd.core.op.keep8 import keep8
 from litenn_amd.core.op.matmul import matmul
 from litenn_amd.core.op.reduce import reduce_mean, reduce_sum
 from litenn_amd.core.op.reshape import flatten, reshape
@@ -45,6 +47,7 @@ from litenn_amd.core.module.Conv2DTranspose import Conv2DTranspose
 from litenn_amd.core.module.DepthwiseConv2D import DepthwiseConv2D
 from litenn_amd.core.module.SeparableConv2D import SeparableConv2D
 from litenn_amd.core.module.Dense import Dense
+from litenn_amd.core.module.GroupNorm import GroupNorm
 
 import litenn_amd.core.optimizer as optimizer
 

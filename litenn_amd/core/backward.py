@@ -4,6 +4,7 @@ import numpy as np
 
 import litenn_amd as nn
 import litenn_amd.core as nc
+from .hip import HipBuffer
 
 _seq = operator.methodcaller('_get_seq_id')
 
@@ -12,12 +13,20 @@ _seq = operator.methodcaller('_get_seq_id')
 # (None outside one) and callbacks run when the gradient functions of the tensor being visited are done, so nothing
 # computed from one sweep's gradients is reused by the next and nothing keeps gradient-sized tensors alive longer
 # than their readers.
-_sweep = {'id': 0, 'active': None, 'tensor_cleanups': []}
+_sweep = {'id': 0, 'active': None, 'tensor_cleanups': [], 'blocked': {}}
 
 
 def current_sweep():
     """Identifier of the backward() call in progress, or None outside one."""
     return _sweep['active']
+
+
+def gradient_wanted(output_t, input_t):
+    """Whether the running backward() asks for input_t's gradient through output_t: a gradient function that forms
+    several inputs' gradients in one pass then forms those that are wanted, and no others."""
+    if output_t._is_freezed() and input_t._is_trainable():
+        return False
+    return input_t._get_seq_id() not in _sweep['blocked']
 
 
 def after_gradfns_of_tensor(fn):
@@ -34,6 +43,7 @@ def _run_tensor_cleanups():
     fns, _sweep['tensor_cleanups'] = _sweep['tensor_cleanups'], []
     for fn in fns:
         fn()
+    HipBuffer.release_decoded()
 
 
 
@@ -59,6 +69,7 @@ def backward(loss, stop_grad=None, grad_for_non_trainables=False, keep_gradient_
     finally:
         _run_tensor_cleanups()
         _sweep['active'] = None
+        _sweep['blocked'] = {}
 
 
 def _backward(loss, stop_grad, grad_for_non_trainables):
@@ -76,6 +87,7 @@ def _backward(loss, stop_grad, grad_for_non_trainables):
     blocked = _untrainable_branches(loss) if not grad_for_non_trainables else {}
     for t in stop_grad:
         blocked[t._get_seq_id()] = []
+    _sweep['blocked'] = blocked
 
     roots = [t for t in loss if t._get_seq_id() not in blocked]
     for t in roots:
@@ -98,9 +110,7 @@ def _backward(loss, stop_grad, grad_for_non_trainables):
         fns = t._get_gradfns()
         if fns is not None:
             for input_t, funcs in fns.items():
-                if t._is_freezed() and input_t._is_trainable():
-                    continue
-                if input_t._get_seq_id() in blocked:
+                if not gradient_wanted(t, input_t):
                     continue
                 for func in funcs:
                     func(t, t.get_grad())

@@ -1,3 +1,5 @@
+import weakref
+
 import numpy as np
 
 from . import api
@@ -12,13 +14,15 @@ class HipBuffer:
      size        bytes
      init_func   callable(HipBuffer) run right after physical allocation
     """
-    __slots__ = ['device', 'size', 'init_func', '_ptr', '_version', '_derived', '__weakref__']
+    __slots__ = ['device', 'size', 'init_func', '_ptr', '_version', '_derived', '_kept', '__weakref__']
     _object_count = 0
+    _decoded = weakref.WeakSet()   # buffers whose fp32 form was made again from their 8-bit copy; release_decoded() empties it
 
     def __init__(self, device, size, init_func=None):
         HipBuffer._object_count += 1
         self._ptr = None
         self._version = 0      # grows whenever the contents may have changed (any access that is not read-only)
+        self._kept = None      # HipBuffer with the contents in 8 bits (keep8), as long as nothing was written since
         self._derived = None   # {key: (version, HipBuffer)}: copies in another layout, valid for that version only
         if size <= 0:
             raise ValueError(f'Create HipBuffer with {size} size.')
@@ -39,12 +43,61 @@ class HipBuffer:
         readonly=True is a promise not to write through the pointer; every other access counts as a change of
         the contents and invalidates copies derived from them (see derived())."""
         if self._ptr is None:
-            self._ptr = self.device._mem_alloc(self.size)
-            if self.init_func is not None and not skip_init:
-                self.init_func(self)
+            if self._kept is not None and not skip_init:
+                self._decode()
+            else:
+                self._ptr = self.device._mem_alloc(self.size)
+                if self.init_func is not None and not skip_init:
+                    self.init_func(self)
         if not readonly:
             self._version += 1
+            self._kept = None
         return self._ptr
+
+    def keep8(self, kept=None):
+        """From here on hold the contents (fp32 values) in 8 bits, rounded; the fp32 memory goes back to the pool.  The
+        next reader that needs fp32 gets it decoded (get_ptr), a writer ends the 8-bit state.  kept: a HipBuffer that a
+        kernel has already filled with the copy."""
+        if ShallowMode.active():
+            return
+        if kept is None and self._kept is None:
+            src = self.get_ptr(readonly=True)
+            kept = HipBuffer(self.device, api.bytes8(self.size // 4))
+            api.encode8(self.device.index, self.size // 4, src, kept.get_ptr(skip_init=True))
+        if kept is not None:
+            self._kept = kept
+            self._version += 1
+            self._derived = None
+        self._free_memory()
+
+    def kept8(self):
+        """The HipBuffer with the contents in 8 bits, or None if they are not held that way."""
+        return self._kept
+
+    def _decode(self):
+        ptr = self.device._mem_alloc(self.size)
+        try:
+            api.decode8(self.device.index, self.size // 4, self._kept.get_ptr(readonly=True), ptr)
+        except Exception:
+            self.device._mem_free(ptr, self.size)
+            raise
+        self._ptr = ptr
+        HipBuffer._decoded.add(self)
+
+    @staticmethod
+    def release_decoded():
+        """Let go of fp32 memory that was filled from 8-bit copies and is not needed past this point: backward() calls it
+        when the gradient functions of a tensor have run, so that the activations of a net are decoded one after the
+        other and never all stand in fp32 together."""
+        for buf in tuple(HipBuffer._decoded):
+            if buf._kept is not None:
+                buf._free_memory()
+        HipBuffer._decoded.clear()
+
+    def _free_memory(self):
+        if self._ptr is not None:
+            self.device._mem_free(self._ptr, self.size)
+            self._ptr = None
 
     def derived(self, key, size, make):
         """A buffer computed from this one's current contents (the weights in a kernel's own layout), kept until
@@ -62,9 +115,8 @@ class HipBuffer:
 
     def free_ptr(self):
         self._derived = None
-        if self._ptr is not None:
-            self.device._mem_free(self._ptr, self.size)
-            self._ptr = None
+        self._kept = None
+        self._free_memory()
 
     def set(self, value):
         """Copy from another HipBuffer (same size) or from an np.ndarray whose

@@ -98,3 +98,19 @@ def permuted_weights(kernel_t, desc, w_layout=api.W_OIHW):
         dev = buf.device.index
         out.append(buf.derived(key, size, lambda src, dst, dev=dev: api.conv2d_permute_weights(dev, desc, src, w_layout, dst)))
     return _BufferList(out)
+
+
+def kept8(t):
+    """The 8-bit copies that tensor t's contents are held in (nn.keep8), as a launch() argument, or None."""
+    copies = [buf.kept8() for buf in t._get_buffers()]
+    return None if any(c is None for c in copies) else _BufferList(copies)
+
+
+def new_kept8(t):
+    """Unfilled buffers for t's 8-bit copies, one per device; hold8(t, them) once a launch has written them."""
+    return _BufferList([HipBuffer(buf.device, api.bytes8(buf.size // 4)) for buf in t._get_buffers()])
+
+
+def hold8(t, copies):
+    for buf, kept in zip(t._get_buffers(), copies._get_buffers()):
+        buf.keep8(kept)

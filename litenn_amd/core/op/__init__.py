@@ -26,6 +26,8 @@ from .dual_wise_op import (dual_wise_op,
                            add_op as add,
                            sub_op as sub,
                            mul_op as mul)
+from .group_norm import group_norm
+from .keep8 import check_keep8, keep8
 from .matmul import (matmul_op as matmul,
                      matmulc_op as matmulc,
                      matmul_bias_act)

@@ -105,7 +105,7 @@ class _EpilogueGrad:
             if current_sweep() is not None:
                 self.key = (current_sweep(), dO_t)
                 after_gradfns_of_tensor(self._drop)
-        args = [O_t, dO_t]
+        args = [(O_t, 'r'), (dO_t, 'r')]     # read only: an output held in 8 bits (nn.keep8) stays so
         if pre is not None:
             args.append((pre, 'w'))
         beta = 0

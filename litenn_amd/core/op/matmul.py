@@ -1,6 +1,6 @@
 import litenn_amd as nn
 import litenn_amd.core as nc
-from ..hip import api, launch
+from ..hip import api, kept8, launch
 
 
 def matmul_op(a_t, b_t, output_t=None, is_add_to_output=False):
@@ -78,10 +78,14 @@ def matmulc_op(a_t, b_t, output_t=None, is_add_to_output=False):
 
 def matmul_a_grad(a_t, b_t, dO_t):
     """a.grad[K][M] += b[N][K]^T . dO[N][M]   (matmul.py:64-67); the transposed
-    operand is read in place, not materialised."""
+    operand is read in place, not materialised - in 8 bits where b is held that way (nn.keep8)."""
     op = nc.Cacheton.get(_MatmulOp, a_t.shape, b_t.shape, False)
     B, M, N, K = op.BATCH, op.M, op.N, op.K
     grad_t, beta = nc.op.accumulate_target(a_t.get_grad())
+    b8 = kept8(b_t)
+    if b8 is not None:
+        launch(lambda dev, x8, do, da: api.gemm_wgrad8(dev, B, N, K, M, x8, do, da, beta), (b8, 'r'), (dO_t, 'r'), grad_t)
+        return
     launch(lambda dev, b, do, da: api.gemm(dev, 1, 0, B, K, M, N, b, K, N * K, do, M, N * M, da, M, K * M, beta),
            (b_t, 'r'), (dO_t, 'r'), grad_t)
 
