@@ -110,7 +110,8 @@ def check(api, seed, N, C, HW, groups, last, name, slope=0.1, eps=1e-5, kept=Fal
 SHAPES = [  # N, C, HW, groups
     (1, 1, 3, 1), (1, 8, 1, 1), (1, 64, 196, 8), (2, 6, 35, 3), (3, 60, 37 * 41, 12), (2, 32, 64, 32), (1, 4, 63, 2), (5, 12, 9, 4),
     (2, 128, 56 * 56, 32), (1, 3, 1000, 1), (4, 96, 49, 8), (2, 320, 256, 32), (1, 16, 70 * 71, 1), (2, 40, 33, 5), (7, 24, 1, 3),
-    (300, 96, 1, 4), (33, 512, 1, 32), (64, 1000, 1, 1), (9, 34, 2, 17), (2, 1028, 5, 4), (1, 2, 65536, 2), (1, 64, 16384, 2)]
+    (300, 96, 1, 4), (33, 512, 1, 32), (64, 1000, 1, 1), (9, 34, 2, 17), (2, 1028, 5, 4), (1, 2, 65536, 2), (1, 64, 16384, 2),
+    (600, 8, 4, 2), (5, 2048, 1, 1), (3, 5000, 1, 1), (2, 20000, 1, 2), (3, 6, 90000, 3), (2, 8000, 3, 1), (1, 33, 70000, 1), (1, 2080, 40, 5)]
 
 
 @pytest.mark.parametrize('shape', SHAPES)
