@@ -60,4 +60,53 @@ __device__ __forceinline__ uint32_t encode_lane4(const float* v, uint32_t* byte)
   return pack4(code_of(v[0], inv), code_of(v[1], inv), code_of(v[2], inv), code_of(v[3], inv));
 }
 
+// Four elements of x (or fewer at the end of a plane: cnt), from fp32 memory or from the 8-bit copy.
+struct SrcF {
+  const float* x;
+  __device__ __forceinline__ void load(uint32_t at, int cnt, float* v) const { load4(x, at, cnt, v); }
+  static __device__ __forceinline__ void load4(const float* p, uint32_t at, int cnt, float* v) {
+    if (cnt == 4) {
+      const F4 f = *reinterpret_cast<const F4*>(p + at);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = f.v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = k < cnt ? p[at + k] : 0.0f;
+    }
+  }
+};
+struct Src8 {
+  const uint8_t* codes;
+  const uint8_t* bytes;
+  __device__ __forceinline__ void load(uint32_t at, int cnt, float* v) const {
+    uint32_t q = 0;
+    if (cnt == 4) {
+      q = reinterpret_cast<const B4*>(codes + at)->v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q |= k < cnt ? (uint32_t)codes[at + k] << (8 * k) : 0u;
+    }
+    if (cnt > 0) {   // four elements lie in one block, or in two
+      const float s0 = step_of(bytes[at >> 5]), s1 = step_of(bytes[(at + cnt - 1) >> 5]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = code_at(q, k) * (((at + k) >> 5) == (at >> 5) ? s0 : s1);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = 0.0f;
+    }
+  }
+};
+__device__ __forceinline__ void store4(float* p, uint32_t at, int cnt, const float* v) {
+  if (cnt == 4) {
+    F4 f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.v[k] = v[k];
+    *reinterpret_cast<F4*>(p + at) = f;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < cnt) p[at + k] = v[k];
+  }
+}
+
 }  // namespace lnn

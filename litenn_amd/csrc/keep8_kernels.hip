@@ -1,5 +1,7 @@
 // Activations kept in 8 bits: writing them, reading them back, and the weight gradient of a dense layer from its kept
 // input.  The element format is in keep8.hpp.
+#include <algorithm>
+
 #include "keep8.hpp"
 
 namespace lnn {
@@ -64,53 +66,253 @@ int launch_decode8(DeviceCtx* ctx, uint64_t n, const void* src, float* dst) {
   return LNN_OK;
 }
 
-// dW[b][k][m] (+)= sum over rows of X8[b][row][k] dO[b][row][m], 64 x 64 outputs per block, 4 x 4 per thread,
-// 16 rows at a time through LDS.
-__global__ __launch_bounds__(256) void wgrad8_kernel(int rows, int K, int M, uint32_t blocks, const uint8_t* x8, const float* dO,
-                                                     float* dW, int beta) {
-  __shared__ float xs[16][64], ds[16][64];
-  const uint8_t* bytes = x8 + (uint64_t)blocks * 32;
-  const int b = blockIdx.z, k0 = blockIdx.y * 64, m0 = blockIdx.x * 64, t = threadIdx.x;
-  const uint32_t xbase = (uint32_t)b * rows * K;
-  const float* d = dO + (uint64_t)b * rows * M;
-  float acc[4][4] = {};
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    for (int i = t; i < 16 * 64; i += 256) {
-      const int r = r0 + (i >> 6), c = i & 63;
-      float xv = 0.0f, dv = 0.0f;
-      if (r < rows && k0 + c < K) {
-        const uint32_t at = xbase + (uint32_t)r * K + k0 + c;
-        xv = (float)(int8_t)x8[at] * step_of(bytes[at >> 5]);
+// ---- weight gradient from a kept input -------------------------------------------------------------------------------
+//
+//   dW[k][m] = sum over rows of X8[row][k] dO[row][m]
+//
+// A kept value is exactly a bf16 number, and dO is exactly the sum of three: h holds the top 8 of its 24 bits, l the
+// last 8, m those between (each cut off, so that all three have dO's sign).  So dW = X8^T h + X8^T m + X8^T l on the bf16 matrix
+// pipe, every product exact and every sum fp32: what an fp32 product of the same values would give, at three times the
+// bf16 work, which is a fifth of the fp32 pipe's time.
+//
+// First pass: both operands are laid out as the matrix instruction reads them, 1 KB per fragment of 32 columns x 16 rows
+// (lane l holds column l % 32, rows 8 (l / 32) .. + 7), rows and columns padded with zeros to whole tiles.  The main kernel
+// then copies fragments to LDS and reads them back without any index arithmetic, bank conflict or bounds check.
+using bf16x8 = __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16;
+using f32x16w = __attribute__((__vector_size__(16 * sizeof(float)))) float;
+typedef __attribute__((address_space(3))) void* lds_void;
+typedef const __attribute__((address_space(1))) void* glb_void;
+
+struct W8 {
+  int rows, K, M, batch;   // rows, batch: of this launch's part
+  int b0, r0, all;         // its first batch item and row; rows of the whole operand
+  int steps;               // of 32 rows
+  int ipan, jpan;    // panels of 32 columns of X and dO, whole tiles
+  uint32_t xblocks;  // of the 8-bit copy
+};
+
+__device__ __forceinline__ uint32_t hi16(uint32_t lo, uint32_t hi) { return (lo >> 16) | (hi & 0xffff0000u); }   // two bf16 of two fp32
+
+// A workgroup lays out 16 rows x 512 columns of X (its first xwgs pieces of 16 rows) or dO at a time; a thread 8 rows x 4
+// columns.
+__device__ __forceinline__ void w8_pack(const W8& w, int b, int r16, bool isx, int pan, const uint8_t* x8, const float* dO, uint4* ap,
+                                        uint4* bp) {
+  const int half = (threadIdx.x >> 3) & 1, quad = threadIdx.x & 7;
+  const int pans = isx ? w.ipan : w.jpan, cols = isx ? w.K : w.M;
+  const int c = pan * 32 + quad * 4, cnt = min(max(cols - c, 0), 4), r0 = r16 * 16 + half * 8;
+  float v[8][4];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const int n = r0 + r < w.rows ? cnt : 0;
+    const uint32_t at = ((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * cols + c;
+    if (isx)
+      Src8{x8, x8 + (uint64_t)w.xblocks * 32}.load(at, n, v[r]);
+    else
+      SrcF::load4(dO, at, n, v[r]);
+  }
+  const uint64_t frag = ((uint64_t)b * 2 * w.steps + r16) * pans + pan;
+  const int lane = half * 32 + quad * 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t h[8], m[8], l[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      h[r] = __float_as_uint(v[r][k]);
+      if (!isx) {
+        const bool odd = (h[r] & 0x7f800000u) == 0x7f800000u;   // infinity and NaN have no rest
+        const float rest = odd ? 0.0f : v[r][k] - __uint_as_float(h[r] & 0xffff0000u);
+        if (odd && (h[r] & 0x7fffffu)) h[r] = 0x7fc00000u;
+        m[r] = __float_as_uint(rest);
+        l[r] = __float_as_uint(rest - __uint_as_float(m[r] & 0xffff0000u));
       }
-      if (r < rows && m0 + c < M) dv = d[(uint64_t)r * M + m0 + c];
-      xs[i >> 6][c] = xv;
-      ds[i >> 6][c] = dv;
     }
-    __syncthreads();
-    for (int r = 0; r < 16; ++r)
+    if (isx) {
+      ap[frag * 64 + lane + k] = make_uint4(hi16(h[0], h[1]), hi16(h[2], h[3]), hi16(h[4], h[5]), hi16(h[6], h[7]));
+    } else {
+      uint4* o = bp + frag * 192 + lane + k;
+      o[0] = make_uint4(hi16(h[0], h[1]), hi16(h[2], h[3]), hi16(h[4], h[5]), hi16(h[6], h[7]));
+      o[64] = make_uint4(hi16(m[0], m[1]), hi16(m[2], m[3]), hi16(m[4], m[5]), hi16(m[6], m[7]));
+      o[128] = make_uint4(hi16(l[0], l[1]), hi16(l[2], l[3]), hi16(l[4], l[5]), hi16(l[6], l[7]));
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void w8_pack_kernel(W8 w, int xwgs, int owgs, const uint8_t* x8, const float* dO, uint4* ap, uint4* bp) {
+  const uint32_t wgs = xwgs + owgs, pieces = (uint32_t)w.batch * 2 * w.steps * wgs;
+  for (uint32_t u = blockIdx.x; u < pieces; u += gridDim.x) {
+    const uint32_t k = u / wgs, y = u - k * wgs;
+    const bool isx = y < (uint32_t)xwgs;
+    const int pan = (isx ? y : y - xwgs) * 16 + threadIdx.x / 16;
+    if (pan < (isx ? w.ipan : w.jpan)) w8_pack(w, k / (2 * w.steps), k % (2 * w.steps), isx, pan, x8, dO, ap, bp);
+  }
+}
+
+// PI x PJ fragments per wavefront, WI x WJ wavefronts: a tile of 32 PI WI (columns of X) x 32 PJ WJ (columns of dO).  A step
+// is 32 rows = two fragments deep; its fragments come into one half of LDS while the other half is multiplied.
+// Output t of the launch's tiles x splits: splits outermost, then groups of eight tile rows, column by column, and the
+// workgroups of one XCD (every eighth) take a contiguous run of t, so that its L2 serves each fragment to several tiles.
+template <int PI, int PJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ) void w8_kernel(W8 w, int ti, int tj, int splits, int per, const uint4* ap, const uint4* bp,
+                                                          float* out, int beta) {
+  constexpr int NI = PI * WI, NJ = PJ * WJ, NW = WI * WJ, FR = 2 * (NI + 3 * NJ), LPW = FR / NW;
+  static_assert(FR % NW == 0, "whole fragments per wavefront");
+  __shared__ uint4 lds[2][FR][64];
+  const int total = ti * tj * splits * w.batch;
+  const int t = (int)(blockIdx.x & 7) * ((total + 7) / 8) + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= (total + 7) / 8 || t >= total) return;
+  const int tiles = ti * tj, tile = t % tiles, z = t / tiles, split = z % splits, b = z / splits;
+  const int grp = tile / (8 * tj), rem = tile - grp * 8 * tj, gi = min(8, ti - grp * 8);
+  const int it = grp * 8 + rem % gi, jt = rem / gi;
+  const int s0 = split * per, s1 = min(s0 + per, w.steps);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wi = wave / WJ, wj = wave % WJ;
+
+  // this wavefront's fragments of a step: [depth][NI], then [depth][NJ][part]
+  const uint4* src[LPW];
+  uint32_t adv[LPW];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+  for (int e = 0; e < LPW; ++e) {
+    const int f = wave * LPW + e;
+    if (f < 2 * NI) {
+      const int d = f / NI, p = f % NI;
+      src[e] = ap + (((uint64_t)(b * w.steps + s0) * 2 + d) * w.ipan + it * NI + p) * 64 + lane;
+      adv[e] = 2u * w.ipan * 64;
+    } else {
+      const int g = f - 2 * NI, d = g / (3 * NJ), p = g % (3 * NJ);
+      src[e] = bp + ((((uint64_t)(b * w.steps + s0) * 2 + d) * w.jpan + jt * NJ) * 3 + p) * 64 + lane;
+      adv[e] = 6u * w.jpan * 64;
+    }
+  }
+  auto request = [&](int half) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += xs[r][(t >> 4) * 4 + i] * ds[r][(t & 15) * 4 + j];
+    for (int e = 0; e < LPW; ++e) {
+      __builtin_amdgcn_global_load_lds((glb_void)src[e], (lds_void)&lds[half][wave * LPW + e][0], 16, 0, 0);
+      src[e] += adv[e];
+    }
+  };
+  f32x16w acc[PI][PJ];
+#pragma unroll
+  for (int i = 0; i < PI; ++i)
+#pragma unroll
+    for (int j = 0; j < PJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+  if (s0 < s1) request(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    const int half = (s - s0) & 1;
+    if (s + 1 < s1) request(half ^ 1);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      bf16x8 a[PI], v[PJ][3];
+#pragma unroll
+      for (int i = 0; i < PI; ++i) a[i] = __builtin_bit_cast(bf16x8, lds[half][d * NI + wi * PI + i][lane]);
+#pragma unroll
+      for (int j = 0; j < PJ; ++j)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) v[j][p] = __builtin_bit_cast(bf16x8, lds[half][2 * NI + (d * NJ + wj * PJ + j) * 3 + p][lane]);
+#pragma unroll
+      for (int p = 2; p >= 0; --p)
+#pragma unroll
+        for (int j = 0; j < PJ; ++j)
+#pragma unroll
+          for (int i = 0; i < PI; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], v[j][p], acc[i][j], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
+  float* o = out + (uint64_t)(splits > 1 ? t / tiles : b) * w.K * w.M;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < PI; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = k0 + (t >> 4) * 4 + i, m = m0 + (t & 15) * 4 + j;
-      if (k < K && m < M) {
-        float* o = dW + ((uint64_t)b * K + k) * M + m;
-        *o = beta ? *o + acc[i][j] : acc[i][j];
+    for (int j = 0; j < PJ; ++j) {
+      const int m = ((jt * WJ + wj) * PJ + j) * 32 + (lane & 31), k0 = ((it * WI + wi) * PI + i) * 32 + 4 * (lane >> 5);
+      if (m < w.M) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int k = k0 + 8 * (e >> 2) + (e & 3);
+          if (k < w.K) {
+            float* at = o + (uint64_t)k * w.M + m;
+            *at = beta ? *at + acc[i][j][e] : acc[i][j][e];
+          }
+        }
       }
     }
 }
 
-int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta) {
-  const uint64_t blocks = blocks8((uint64_t)batch * rows * K);
-  hipLaunchKernelGGL(wgrad8_kernel, dim3((M + 63) / 64, (K + 63) / 64, batch), dim3(256), 0, ctx->stream, rows, K, M,
-                     (uint32_t)blocks, static_cast<const uint8_t*>(x8), dO, dW, beta);
+// dW (+)= the splits' partial results, in order
+__global__ __launch_bounds__(256) void w8_join_kernel(uint32_t n, int splits, int batch, const float* part, float* dW, int beta) {
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < (uint64_t)n * batch; i += gridDim.x * 256ull) {
+    const uint32_t b = (uint32_t)(i / n), e = (uint32_t)(i - (uint64_t)b * n);
+    const float* p = part + (uint64_t)b * splits * n + e;
+    float s = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) s += p[(uint64_t)k * n];
+    dW[i] = beta ? dW[i] + s : s;
+  }
+}
+
+static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* dO, float* dW, int beta) {
+  const int K = w.K, M = w.M, batch = w.batch;
+  // 256 x 256 tiles once they alone give most compute units one, else 128 x 128 ones
+  auto tiles = [&](int side) { return (int64_t)((K + side - 1) / side) * ((M + side - 1) / side) * batch; };
+  const int side = tiles(256) * 4 >= 3 * ctx->cus ? 256 : 128;
+  const int ti = (K + side - 1) / side, tj = (M + side - 1) / side;
+  w.ipan = ti * side / 32;
+  w.jpan = tj * side / 32;
+  // rows split until every compute unit has a tile (128: two), two steps at least to a split
+  const int64_t want = (int64_t)ctx->cus * (side == 256 ? 1 : 2) / tiles(side);
+  int splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, w.steps / 2));
+  const int per = (w.steps + splits - 1) / splits;
+  splits = (w.steps + per - 1) / per;
+  const uint64_t afrag = (uint64_t)batch * 2 * w.steps * w.ipan, bfrag = (uint64_t)batch * 2 * w.steps * w.jpan * 3;
+  const uint64_t part = splits > 1 ? (uint64_t)batch * splits * K * M * 4 : 0;
+  int st = ensure_workspace(ctx, (afrag + bfrag) * 1024 + part);
+  if (st != LNN_OK) return st;
+  uint4* ap = static_cast<uint4*>(ctx->ws);
+  uint4* bp = ap + afrag * 64;
+  float* pp = reinterpret_cast<float*>(bp + bfrag * 64);
+  const int xwgs = (w.ipan + 15) / 16, owgs = (w.jpan + 15) / 16;
+  const uint64_t pieces = (uint64_t)batch * 2 * w.steps * (xwgs + owgs);
+  hipLaunchKernelGGL(w8_pack_kernel, dim3((unsigned)std::min<uint64_t>(pieces, 1u << 20)), dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO,
+                     ap, bp);
+  const int64_t total = (int64_t)ti * tj * splits * batch;
+  const dim3 grid((unsigned)((total + 7) / 8 * 8));
+  float* out = splits > 1 ? pp : dW;
+  const int b0 = splits > 1 ? 0 : beta;
+  if (side == 256)
+    hipLaunchKernelGGL((w8_kernel<4, 2, 2, 4>), grid, dim3(512), 0, ctx->stream, w, ti, tj, splits, per, ap, bp, out, b0);
+  else
+    hipLaunchKernelGGL((w8_kernel<2, 2, 2, 2>), grid, dim3(256), 0, ctx->stream, w, ti, tj, splits, per, ap, bp, out, b0);
+  if (splits > 1)
+    hipLaunchKernelGGL(w8_join_kernel, grid8(ctx, (uint64_t)K * M * batch), dim3(256), 0, ctx->stream, (uint32_t)K * M, splits, batch, pp, dW, beta);
   LNN_HIP(hipGetLastError());
+  return LNN_OK;
+}
+
+int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta) {
+  W8 w = {};
+  w.K = K;
+  w.M = M;
+  w.all = rows;
+  w.xblocks = (uint32_t)blocks8((uint64_t)batch * rows * K);
+  // The laid-out operands of one launch stay below a gigabyte: many small products go in groups, one product of very
+  // many rows in runs of rows, each added to the one before.
+  const uint64_t step = ((uint64_t)((K + 255) / 256) + 3 * (uint64_t)((M + 255) / 256)) * 16384;   // bytes of 32 rows, at most
+  const int64_t most = std::max<int64_t>(1, (int64_t)((1u << 30) / step));                         // steps of one launch
+  const int64_t steps = ((int64_t)rows + 31) / 32;
+  const int group = (int)std::min<int64_t>(batch, std::max<int64_t>(1, most / steps));
+  const int run = (int)std::min<int64_t>(rows, most * 32);
+  for (w.b0 = 0; w.b0 < batch; w.b0 += group)
+    for (w.r0 = 0;; w.r0 += run) {
+      w.batch = std::min(group, batch - w.b0);
+      w.rows = std::min(run, rows - w.r0);
+      w.steps = (w.rows + 31) / 32;
+      int st = wgrad8_part(ctx, w, static_cast<const uint8_t*>(x8), dO, dW + (uint64_t)w.b0 * K * M, w.r0 > 0 ? 1 : beta);
+      if (st != LNN_OK) return st;
+      if (run >= rows - w.r0) break;
+    }
   return LNN_OK;
 }
 
