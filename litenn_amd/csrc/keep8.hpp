@@ -60,39 +60,68 @@ __device__ __forceinline__ uint32_t encode_lane4(const float* v, uint32_t* byte)
   return pack4(code_of(v[0], inv), code_of(v[1], inv), code_of(v[2], inv), code_of(v[3], inv));
 }
 
-// Four elements of x (or fewer at the end of a plane: cnt), from fp32 memory or from the 8-bit copy.
-struct SrcF {
-  const float* x;
-  __device__ __forceinline__ void load(uint32_t at, int cnt, float* v) const { load4(x, at, cnt, v); }
-  static __device__ __forceinline__ void load4(const float* p, uint32_t at, int cnt, float* v) {
-    if (cnt == 4) {
-      const F4 f = *reinterpret_cast<const F4*>(p + at);
+// Four elements of a tensor at any place, of which the first cnt count; the others are set to 0.  No branch: behind one,
+// the compiler waits for each load before it sends the next, and a kernel that holds a row in registers has nothing else
+// to cover that latency (backward pass of 32 x 128 x 56 x 56: 39 us with branches).  Lanes without elements read the
+// tensor's start; groups that hang over its end read its last four elements and shift.
+//   G4      every group is whole (cnt 0 or 4)
+//   GANY    any cnt, tensor of four elements or more
+//   GTINY   any cnt, any tensor: element by element
+// size: elements of the tensor.
+enum { G4, GANY, GTINY };
+template <int MODE>
+__device__ __forceinline__ void load4(const float* p, uint32_t at, int cnt, uint32_t size, float* v) {
+  if (MODE == GTINY) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = f.v[k];
-    } else {
+    for (int k = 0; k < 4; ++k) v[k] = p[min(at + k, size - 1)];
+  } else {
+    const uint32_t from = cnt > 0 ? (MODE == GANY ? min(at, size - 4) : at) : 0u;
+    const F4 f = *reinterpret_cast<const F4*>(p + from);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = k < cnt ? p[at + k] : 0.0f;
+    for (int k = 0; k < 4; ++k) v[k] = f.v[k];
+    if (MODE == GANY) {
+      const uint32_t d = at - from;
+      if (d & 1) { v[0] = v[1]; v[1] = v[2]; v[2] = v[3]; }
+      if (d & 2) { v[0] = v[2]; v[1] = v[3]; }
     }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = k < cnt ? v[k] : 0.0f;
+}
+// The codes of four elements as one word (0 where there is none): the codes of a copy are padded to whole blocks.
+template <int MODE>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, uint32_t at, int cnt, uint32_t size) {
+  if (MODE == G4) {
+    const uint32_t q = reinterpret_cast<const B4*>(p + (cnt > 0 ? at : 0u))->v;
+    return cnt > 0 ? q : 0u;
+  }
+  const uint32_t from = cnt > 0 ? min(at, ((size + 31) & ~31u) - 4) : 0u;
+  const uint32_t q = reinterpret_cast<const B4*>(p + from)->v >> (cnt > 0 ? 8 * (at - from) : 0u);
+  return cnt >= 4 ? q : q & ((1u << (8 * max(cnt, 0))) - 1);
+}
+// Sources of x: fp32 memory, or the 8-bit copy
+struct SrcF {
+  const float* x;
+  __device__ __forceinline__ float at(uint32_t i) const { return x[i]; }
+  template <int MODE>
+  __device__ __forceinline__ void load(uint32_t at, int cnt, uint32_t size, float* v) const { load4<MODE>(x, at, cnt, size, v); }
 };
 struct Src8 {
   const uint8_t* codes;
   const uint8_t* bytes;
-  __device__ __forceinline__ void load(uint32_t at, int cnt, float* v) const {
-    uint32_t q = 0;
-    if (cnt == 4) {
-      q = reinterpret_cast<const B4*>(codes + at)->v;
-    } else {
+  __device__ __forceinline__ float at(uint32_t i) const { return (float)(int8_t)codes[i] * step_of(bytes[i >> 5]); }
+  template <int MODE>
+  __device__ __forceinline__ void load(uint32_t at, int cnt, uint32_t size, float* v) const {
+    const uint32_t q = load_codes<MODE>(codes, at, cnt, size);
+    const uint32_t b0 = cnt > 0 ? at >> 5 : 0u;
+    const float s0 = step_of(bytes[b0]);
+    if (MODE == G4) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) q |= k < cnt ? (uint32_t)codes[at + k] << (8 * k) : 0u;
-    }
-    if (cnt > 0) {   // four elements lie in one block, or in two
-      const float s0 = step_of(bytes[at >> 5]), s1 = step_of(bytes[(at + cnt - 1) >> 5]);
+      for (int k = 0; k < 4; ++k) v[k] = code_at(q, k) * s0;
+    } else {   // four elements lie in one block, or in two
+      const float s1 = step_of(bytes[cnt > 0 ? min(at + 3, size - 1) >> 5 : 0u]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = code_at(q, k) * (((at + k) >> 5) == (at >> 5) ? s0 : s1);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = 0.0f;
+      for (int k = 0; k < 4; ++k) v[k] = k < cnt ? code_at(q, k) * (((at + k) >> 5) == b0 ? s0 : s1) : 0.0f;
     }
   }
 };

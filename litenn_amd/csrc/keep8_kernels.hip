@@ -75,6 +75,10 @@ int launch_decode8(DeviceCtx* ctx, uint64_t n, const void* src, float* dst) {
 // pipe, every product exact and every sum fp32: what an fp32 product of the same values would give, at three times the
 // bf16 work, which is a fifth of the fp32 pipe's time.
 //
+// Measured: 8192 rows, 4096 x 4096: 0.72 ms = 1.15 PFLOP/s of bf16 work, 380 TFLOP/s of the product (the fp32 pipe's product of
+// decoded values: 2.0 ms), the main kernel alone 0.63 ms, 1.3 PFLOP/s: as the library's bf16 product of that size runs here.
+// Bound: the matrix pipe; the first pass, 435 MB of traffic, is the rest.
+//
 // First pass: both operands are laid out as the matrix instruction reads them, 1 KB per fragment of 32 columns x 16 rows
 // (lane l holds column l % 32, rows 8 (l / 32) .. + 7), rows and columns padded with zeros to whole tiles.  The main kernel
 // then copies fragments to LDS and reads them back without any index arithmetic, bank conflict or bounds check.
@@ -88,13 +92,14 @@ struct W8 {
   int b0, r0, all;         // its first batch item and row; rows of the whole operand
   int steps;               // of 32 rows
   int ipan, jpan;    // panels of 32 columns of X and dO, whole tiles
-  uint32_t xblocks;  // of the 8-bit copy
+  uint32_t xblocks, xsize, osize;   // blocks of the 8-bit copy; elements of X and dO
 };
 
 __device__ __forceinline__ uint32_t hi16(uint32_t lo, uint32_t hi) { return (lo >> 16) | (hi & 0xffff0000u); }   // two bf16 of two fp32
 
 // A workgroup lays out 16 rows x 512 columns of X (its first xwgs pieces of 16 rows) or dO at a time; a thread 8 rows x 4
 // columns.
+template <int MX, int MO>
 __device__ __forceinline__ void w8_pack(const W8& w, int b, int r16, bool isx, int pan, const uint8_t* x8, const float* dO, uint4* ap,
                                         uint4* bp) {
   const int half = (threadIdx.x >> 3) & 1, quad = threadIdx.x & 7;
@@ -106,9 +111,9 @@ __device__ __forceinline__ void w8_pack(const W8& w, int b, int r16, bool isx, i
     const int n = r0 + r < w.rows ? cnt : 0;
     const uint32_t at = ((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * cols + c;
     if (isx)
-      Src8{x8, x8 + (uint64_t)w.xblocks * 32}.load(at, n, v[r]);
+      Src8{x8, x8 + (uint64_t)w.xblocks * 32}.load<MX>(at, n, w.xsize, v[r]);
     else
-      SrcF::load4(dO, at, n, v[r]);
+      load4<MO>(dO, at, n, w.osize, v[r]);
   }
   const uint64_t frag = ((uint64_t)b * 2 * w.steps + r16) * pans + pan;
   const int lane = half * 32 + quad * 4;
@@ -137,13 +142,14 @@ __device__ __forceinline__ void w8_pack(const W8& w, int b, int r16, bool isx, i
   }
 }
 
+template <int MX, int MO>
 __global__ __launch_bounds__(256) void w8_pack_kernel(W8 w, int xwgs, int owgs, const uint8_t* x8, const float* dO, uint4* ap, uint4* bp) {
   const uint32_t wgs = xwgs + owgs, pieces = (uint32_t)w.batch * 2 * w.steps * wgs;
   for (uint32_t u = blockIdx.x; u < pieces; u += gridDim.x) {
     const uint32_t k = u / wgs, y = u - k * wgs;
     const bool isx = y < (uint32_t)xwgs;
     const int pan = (isx ? y : y - xwgs) * 16 + threadIdx.x / 16;
-    if (pan < (isx ? w.ipan : w.jpan)) w8_pack(w, k / (2 * w.steps), k % (2 * w.steps), isx, pan, x8, dO, ap, bp);
+    if (pan < (isx ? w.ipan : w.jpan)) w8_pack<MX, MO>(w, k / (2 * w.steps), k % (2 * w.steps), isx, pan, x8, dO, ap, bp);
   }
 }
 
@@ -253,7 +259,8 @@ __global__ __launch_bounds__(256) void w8_join_kernel(uint32_t n, int splits, in
   }
 }
 
-static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* dO, float* dW, int beta) {
+// need: where to leave the scratch bytes of this part instead of launching it, or null
+static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* dO, float* dW, int beta, uint64_t* need) {
   const int K = w.K, M = w.M, batch = w.batch;
   // 256 x 256 tiles once they alone give most compute units one, else 128 x 128 ones
   auto tiles = [&](int side) { return (int64_t)((K + side - 1) / side) * ((M + side - 1) / side) * batch; };
@@ -268,15 +275,24 @@ static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* 
   splits = (w.steps + per - 1) / per;
   const uint64_t afrag = (uint64_t)batch * 2 * w.steps * w.ipan, bfrag = (uint64_t)batch * 2 * w.steps * w.jpan * 3;
   const uint64_t part = splits > 1 ? (uint64_t)batch * splits * K * M * 4 : 0;
-  int st = ensure_workspace(ctx, (afrag + bfrag) * 1024 + part);
-  if (st != LNN_OK) return st;
+  if (need) {
+    *need = (afrag + bfrag) * 1024 + part;
+    return LNN_OK;
+  }
   uint4* ap = static_cast<uint4*>(ctx->ws);
   uint4* bp = ap + afrag * 64;
   float* pp = reinterpret_cast<float*>(bp + bfrag * 64);
   const int xwgs = (w.ipan + 15) / 16, owgs = (w.jpan + 15) / 16;
   const uint64_t pieces = (uint64_t)batch * 2 * w.steps * (xwgs + owgs);
-  hipLaunchKernelGGL(w8_pack_kernel, dim3((unsigned)std::min<uint64_t>(pieces, 1u << 20)), dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO,
-                     ap, bp);
+  const dim3 pgrid((unsigned)std::min<uint64_t>(pieces, 1u << 20));
+  // rows of whole groups of four are read without shifts; dO of fewer than four elements one by one
+  const bool x4 = K % 4 == 0, o4 = M % 4 == 0;
+  if (w.osize < 4)
+    hipLaunchKernelGGL((w8_pack_kernel<GANY, GTINY>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
+  else if (x4 && o4)
+    hipLaunchKernelGGL((w8_pack_kernel<G4, G4>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
+  else
+    hipLaunchKernelGGL((w8_pack_kernel<GANY, GANY>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
   const int64_t total = (int64_t)ti * tj * splits * batch;
   const dim3 grid((unsigned)((total + 7) / 8 * 8));
   float* out = splits > 1 ? pp : dW;
@@ -296,7 +312,9 @@ int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void*
   w.K = K;
   w.M = M;
   w.all = rows;
-  w.xblocks = (uint32_t)blocks8((uint64_t)batch * rows * K);
+  w.xsize = (uint32_t)batch * rows * K;
+  w.osize = (uint32_t)batch * rows * M;
+  w.xblocks = (uint32_t)blocks8(w.xsize);
   // The laid-out operands of one launch stay below a gigabyte: many small products go in groups, one product of very
   // many rows in runs of rows, each added to the one before.
   const uint64_t step = ((uint64_t)((K + 255) / 256) + 3 * (uint64_t)((M + 255) / 256)) * 16384;   // bytes of 32 rows, at most
@@ -304,15 +322,25 @@ int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void*
   const int64_t steps = ((int64_t)rows + 31) / 32;
   const int group = (int)std::min<int64_t>(batch, std::max<int64_t>(1, most / steps));
   const int run = (int)std::min<int64_t>(rows, most * 32);
-  for (w.b0 = 0; w.b0 < batch; w.b0 += group)
-    for (w.r0 = 0;; w.r0 += run) {
-      w.batch = std::min(group, batch - w.b0);
-      w.rows = std::min(run, rows - w.r0);
-      w.steps = (w.rows + 31) / 32;
-      int st = wgrad8_part(ctx, w, static_cast<const uint8_t*>(x8), dO, dW + (uint64_t)w.b0 * K * M, w.r0 > 0 ? 1 : beta);
+  // Scratch for the largest part comes first: a call that runs out of memory has not written or added anything yet.
+  uint64_t most_bytes = 0;
+  for (int launch = 0; launch < 2; ++launch) {
+    for (w.b0 = 0; w.b0 < batch; w.b0 += group)
+      for (w.r0 = 0;; w.r0 += run) {
+        w.batch = std::min(group, batch - w.b0);
+        w.rows = std::min(run, rows - w.r0);
+        w.steps = (w.rows + 31) / 32;
+        uint64_t need = 0;
+        int st = wgrad8_part(ctx, w, static_cast<const uint8_t*>(x8), dO, dW + (uint64_t)w.b0 * K * M, w.r0 > 0 ? 1 : beta, launch ? nullptr : &need);
+        if (st != LNN_OK) return st;
+        most_bytes = std::max(most_bytes, need);
+        if (run >= rows - w.r0) break;
+      }
+    if (!launch) {
+      int st = ensure_workspace(ctx, most_bytes);
       if (st != LNN_OK) return st;
-      if (run >= rows - w.r0) break;
     }
+  }
   return LNN_OK;
 }
 

@@ -17,19 +17,17 @@ namespace lnn {
 struct NormGeom {
   int N, C, HW, G, Cg, last, silu;
   int n0, nb;           // images of this launch
-  float slope, eps, inv_d;
-  uint32_t D, row0;   // row0: first row of this launch (a grid holds fewer than 2^32 threads)
+  float slope, eps;
+  float d, inv_d;       // D and 1 / D; means are divided by D: a row of equal values then has exactly their mean
+  uint32_t D, size;   // elements of a row and of the tensor
+  uint32_t row0;      // row0: first row of this launch (a grid holds fewer than 2^32 threads)
 };
 
-// 1 / (1 + exp(-p)).  v_exp_f32 takes powers of two: -p log2(e) is rounded, and what the rounding lost goes back in to
-// first order (without it the error grows with |p|).  Beyond 2^126 the sigmoid is 0 next to any p a row can hold.
+// 1 / (1 + exp(-p)) by the one-instruction power of two and reciprocal (one unit in the last place each).  Rounding
+// -p log2(e) costs |p| 2^-25 of exp(-p) besides: 2e-7 at |p| = 5, and where |p| is large the result is next to 0 or 1.
+// The library's expf and a full division take five times the vector work, and these kernels then wait for it, not for memory.
 __device__ __forceinline__ float sigmoid(float p) {
-  constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
-  const float t = fminf(-p * kLog2e, 126.0f);
-  const float lo = fmaf(-p, kLog2e, -t);
-  float e = __builtin_amdgcn_exp2f(t);
-  e = fmaf(e, t < 126.0f ? lo * kLn2 : 0.0f, e);
-  return __builtin_amdgcn_rcpf(1.0f + e);
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(p * -1.44269504088896341f));
 }
 // f of four values in place; no activation is a leaky ReLU of slope 1
 __device__ __forceinline__ void act4(int silu, float slope, float* p) {
@@ -47,7 +45,7 @@ __device__ __forceinline__ void slope4(int silu, float slope, const float* p, fl
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float s = sigmoid(p[k]);
-      d[k] *= s * fmaf(p[k], 1.0f - s, 1.0f);
+      d[k] *= fmaf(p[k] * s, 1.0f - s, s);
     }
   } else {
 #pragma unroll
@@ -58,7 +56,10 @@ __device__ __forceinline__ void slope4(int silu, float slope, const float* p, fl
 // ---- a whole row in registers (channels first, row contiguous) ------------------------------------------------------
 //
 // One workgroup per row reads it once: a lane holds V groups of four elements, and mean, variance and result come from
-// registers.  The row is dealt out in units of 2^ul lanes, each unit inside one channel plane (4 * 2^ul elements of it),
+// registers.  512 lanes: two rows or more to a compute unit, so that one is read while another is computed or written
+// (32 x 256 x 56 x 56 from 8 bits, forward + backward: 116 us against 130 with 1024 lanes and one row); 1024 where there are
+// fewer rows than compute units.  The loads of a row stand together, in front of everything that waits for them (67 -> 61 us).
+// Bound: memory.  32 x 128 x 56 x 56 forward 22 us, 4.7 TB/s; forward + backward with SiLU 61 us, 4.2 TB/s.  The row is dealt out in units of 2^ul lanes, each unit inside one channel plane (4 * 2^ul elements of it),
 // so gamma, beta and the channel sums of the backward pass belong to whole units and no element needs a division.
 struct Units {
   int ul, per, total;   // log2 lanes of a unit; units of a plane; units of the row
@@ -70,7 +71,7 @@ struct UnitPos {
 };
 __device__ __forceinline__ UnitPos unit_pos(const NormGeom& q, const Units& un, uint32_t u, uint32_t lane) {
   UnitPos r;
-  r.ch = un.per == 1 ? u : un.dper.div(u);
+  r.ch = un.dper.div(u);
   const uint32_t pix = (((u - r.ch * un.per) << un.ul) + lane) * 4;
   r.at = r.ch * q.HW + pix;
   r.cnt = u < (uint32_t)un.total ? min(max(q.HW - (int)pix, 0), 4) : 0;
@@ -90,35 +91,62 @@ __device__ __forceinline__ float sum_all(float v, float* sh) {   // over the T t
   return s;
 }
 
-template <int T, int V, bool KEEP>
+// Computes a value anew where it is used next, instead of holding it in a register until then.
+__device__ __forceinline__ uint32_t anew(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// gamma and beta of a group in LDS (ones and zeros where there are none): the first T channels' are asked for before the
+// row, so that waiting for them does not wait for it.
+struct Affine {
+  float g, b;
+};
+template <int T>
+__device__ __forceinline__ Affine ask_affine(const NormGeom& q, uint32_t c0, const float* gamma, const float* beta) {
+  const uint32_t ch = min((int)threadIdx.x, q.Cg - 1);
+  return {gamma ? gamma[c0 + ch] : 1.0f, beta ? beta[c0 + ch] : 0.0f};
+}
+template <int T>
+__device__ __forceinline__ void keep_affine(const NormGeom& q, uint32_t c0, const float* gamma, const float* beta, const Affine& a, float* lg) {
+  if ((int)threadIdx.x < q.Cg) {
+    lg[threadIdx.x] = a.g;
+    lg[q.Cg + threadIdx.x] = a.b;
+  }
+  for (int ch = threadIdx.x + T; ch < q.Cg; ch += T) {
+    lg[ch] = gamma ? gamma[c0 + ch] : 1.0f;
+    lg[q.Cg + ch] = beta ? beta[c0 + ch] : 0.0f;
+  }
+}
+
+template <int T, int V, int MODE, bool KEEP>
 __global__ __launch_bounds__(T) void gn_fwd_res_kernel(NormGeom q, Units un, const float* x, const float* gamma, const float* beta,
                                                        float* y, float* mean, float* rstd, uint8_t* codes, uint8_t* bytes) {
+  extern __shared__ float lg[];   // [2][Cg]
   __shared__ float sh[2][T / 64];
   const uint32_t row = q.row0 + blockIdx.x, base = row * q.D, c0 = (row % q.G) * q.Cg;
   const uint32_t lane = threadIdx.x & ((1u << un.ul) - 1), u0 = threadIdx.x >> un.ul;
   const int step = T >> un.ul;
+  const Affine af = ask_affine<T>(q, c0, gamma, beta);
   float v[V][4];
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    if (i * step < un.total) {
-      const UnitPos p = unit_pos(q, un, i * step + u0, lane);
-      SrcF::load4(x, base + p.at, p.cnt, v[i]);
-    }
+    const UnitPos p = unit_pos(q, un, i * step + u0, lane);   // no test whether the units end: the loads stay together
+    load4<MODE>(x, base + p.at, p.cnt, q.size, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    if (i * step < un.total) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += v[i][k];
-    }
+    for (int k = 0; k < 4; ++k) s += v[i][k];
   }
-  const float m = sum_all<T>(s, sh[0]) * q.inv_d;
+  keep_affine<T>(q, c0, gamma, beta, af, lg);
+  const float m = sum_all<T>(s, sh[0]) / q.d;
   s = 0.0f;
+  const uint32_t u1 = anew(u0);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (i * step < un.total) {
-      const UnitPos p = unit_pos(q, un, i * step + u0, lane);
+      const UnitPos p = unit_pos(q, un, i * step + u1, lane);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float d = k < p.cnt ? v[i][k] - m : 0.0f;
@@ -131,10 +159,12 @@ __global__ __launch_bounds__(T) void gn_fwd_res_kernel(NormGeom q, Units un, con
     mean[row] = m;
     rstd[row] = r;
   }
+  const uint32_t u2 = anew(u0);
+  if (T == 64) __syncthreads();   // gamma and beta are in LDS: larger workgroups have passed a barrier since
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (i * step < un.total) {
-      const UnitPos p = unit_pos(q, un, i * step + u0, lane);
+      const UnitPos p = unit_pos(q, un, i * step + u2, lane);
       if (KEEP) {   // planes are whole blocks of 32: the eight lanes of a block are all in or all out
         uint32_t byte;
         const uint32_t code = encode_lane4(v[i], &byte);
@@ -144,7 +174,7 @@ __global__ __launch_bounds__(T) void gn_fwd_res_kernel(NormGeom q, Units un, con
         }
       }
       if (p.cnt > 0) {
-        const float ga = gamma ? gamma[c0 + p.ch] : 1.0f, be = beta ? beta[c0 + p.ch] : 0.0f;
+        const float ga = lg[p.ch], be = lg[q.Cg + p.ch];
         float o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = (v[i][k] - m) * r * ga + be;
@@ -155,48 +185,70 @@ __global__ __launch_bounds__(T) void gn_fwd_res_kernel(NormGeom q, Units un, con
   }
 }
 
+// What a lane keeps of four elements of x between the two uses: the values, or where they lie in one block the codes and
+// their step, which leaves room for twice the rows on a compute unit.
+struct HoldF {
+  float v[4];
+  __device__ __forceinline__ float get(int k) const { return v[k]; }
+};
+struct Hold8 {
+  uint32_t q;
+  float s;
+  __device__ __forceinline__ float get(int k) const { return code_at(q, k) * s; }
+};
+template <int MODE, class SRC>
+__device__ __forceinline__ void hold4(const SRC& x, uint32_t at, int cnt, uint32_t size, HoldF* h) {
+  x.template load<MODE>(at, cnt, size, h->v);
+}
+template <int MODE>
+__device__ __forceinline__ void hold4(const Src8& x, uint32_t at, int cnt, uint32_t size, Hold8* h) {
+  h->q = load_codes<MODE>(x.codes, at, cnt, size);
+  h->s = step_of(x.bytes[cnt > 0 ? at >> 5 : 0u]);
+}
+
 // Both sums of a unit are formed by lane exchanges and left in LDS; the channel sums are theirs in order, so nothing
 // depends on which wavefront came first.  part (or null): [2][N][C], the channel sums of dp and of dp xh.
-template <int T, int V, class SRC>
-__global__ __launch_bounds__(T) void gn_bwd_res_kernel(NormGeom q, Units un, SRC x, const float* gamma, const float* beta,
-                                                       const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx,
-                                                       float* part) {
-  extern __shared__ float su[];   // [units][2]
+template <int T, int V, int MODE, class SRC, class HOLD>
+__global__ __launch_bounds__(T, T == 512 ? 4 : 1) void gn_bwd_res_kernel(NormGeom q, Units un, SRC x, const float* gamma, const float* beta,
+                                                                         const float* mean, const float* rstd, const float* dy, float* dx,
+                                                                         int beta_dx, float* part) {
+  extern __shared__ float su[];   // [units][2], then gamma and beta [2][Cg]
+  float* lg = su + 2 * un.total;
   __shared__ float sh[2][T / 64];
   const uint32_t row = q.row0 + blockIdx.x, base = row * q.D, n = row / q.G, c0 = (row % q.G) * q.Cg;
   const uint32_t lane = threadIdx.x & ((1u << un.ul) - 1), u0 = threadIdx.x >> un.ul;
   const int step = T >> un.ul;
   const float m = mean[row], r = rstd[row];
-  float xh[V][4], dp[V][4];
+  const Affine af = ask_affine<T>(q, c0, gamma, beta);
+  HOLD xv[V];
+  float dp[V][4];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    if (i * step < un.total) {
-      const UnitPos p = unit_pos(q, un, i * step + u0, lane);
-      x.load(base + p.at, p.cnt, xh[i]);
-      SrcF::load4(dy, base + p.at, p.cnt, dp[i]);
-    }
+    const UnitPos p = unit_pos(q, un, i * step + u0, lane);   // no test whether the units end: the loads stay together
+    hold4<MODE>(x, base + p.at, p.cnt, q.size, &xv[i]);
+    load4<MODE>(dy, base + p.at, p.cnt, q.size, dp[i]);
   }
+  keep_affine<T>(q, c0, gamma, beta, af, lg);
+  __syncthreads();
+  const uint32_t u1 = anew(u0);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (i * step < un.total) {
-      const uint32_t u = i * step + u0;
+      const uint32_t u = i * step + u1;
       const UnitPos p = unit_pos(q, un, u, lane);
-      float ga = 1.0f, be = 0.0f;
-      if (p.cnt > 0) {
-        if (gamma) ga = gamma[c0 + p.ch];
-        if (beta) be = beta[c0 + p.ch];
-      }
-      float a = 0.0f, b = 0.0f, pre[4];
+      const uint32_t ch = min(p.ch, (uint32_t)q.Cg - 1);
+      const float ga = lg[ch], be = lg[q.Cg + ch];
+      float a = 0.0f, b = 0.0f, xh[4], pre[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        xh[i][k] = k < p.cnt ? (xh[i][k] - m) * r : 0.0f;
-        pre[k] = xh[i][k] * ga + be;
+        xh[k] = k < p.cnt ? (xv[i].get(k) - m) * r : 0.0f;
+        pre[k] = xh[k] * ga + be;
       }
       slope4(q.silu, q.slope, pre, dp[i]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         a += dp[i][k];
-        b += dp[i][k] * xh[i][k];
+        b += dp[i][k] * xh[k];
         dp[i][k] *= ga;
       }
       for (int w = (1 << un.ul) >> 1; w > 0; w >>= 1) {
@@ -221,23 +273,24 @@ __global__ __launch_bounds__(T) void gn_bwd_res_kernel(NormGeom q, Units un, SRC
       part[n * q.C + c0 + ch] = a;
       part[(uint32_t)(q.N + n) * q.C + c0 + ch] = b;
     }
-    const float ga = gamma ? gamma[c0 + ch] : 1.0f;
+    const float ga = lg[ch];
     s1 += ga * a;
     s2 += ga * b;
   }
   if (!dx) return;
   s1 = sum_all<T>(s1, sh[0]) * q.inv_d;
   s2 = sum_all<T>(s2, sh[1]) * q.inv_d;
+  const uint32_t u2 = anew(u0);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (i * step < un.total) {
-      const UnitPos p = unit_pos(q, un, i * step + u0, lane);
+      const UnitPos p = unit_pos(q, un, i * step + u2, lane);
       if (p.cnt > 0) {
         float o[4];
-        if (beta_dx) SrcF::load4(dx, base + p.at, p.cnt, o);
+        if (beta_dx) load4<MODE>(dx, base + p.at, p.cnt, q.size, o);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float e = r * (dp[i][k] - s1 - xh[i][k] * s2);
+          const float e = r * (dp[i][k] - s1 - (xv[i].get(k) - m) * r * s2);
           o[k] = beta_dx ? o[k] + e : e;
         }
         store4(dx, base + p.at, p.cnt, o);
@@ -249,6 +302,7 @@ __global__ __launch_bounds__(T) void gn_bwd_res_kernel(NormGeom q, Units un, SRC
 // ---- rows of channels alone (HW = 1: behind a dense layer) ----------------------------------------------------------
 //
 // A row is C / groups neighbouring floats: L lanes hold it, V groups of four each, 256 / L rows to a workgroup.
+// 8192 x 4096 in 32 groups, forward + backward: 142 us, 4.8 TB/s of the 5.0 that a large copy reaches.
 template <int L>
 __device__ __forceinline__ float sum_lanes(float v, float* sh) {
 #pragma unroll
@@ -259,7 +313,7 @@ __device__ __forceinline__ float sum_lanes(float v, float* sh) {
   return sh[0] + sh[1] + sh[2] + sh[3];
 }
 
-template <int L, int V, bool KEEP>
+template <int L, int V, int MODE, bool KEEP>
 __global__ __launch_bounds__(256) void gn_fwd_rows_kernel(NormGeom q, const float* x, const float* gamma, const float* beta, float* y,
                                                           float* mean, float* rstd, uint8_t* codes, uint8_t* bytes) {
   __shared__ float sh[2][4];
@@ -271,13 +325,13 @@ __global__ __launch_bounds__(256) void gn_fwd_rows_kernel(NormGeom q, const floa
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     cnt[i] = row < rows ? min(max(q.Cg - (int)(i * L + lane) * 4, 0), 4) : 0;
-    SrcF::load4(x, base + (i * L + lane) * 4, cnt[i], v[i]);
+    load4<MODE>(x, base + (i * L + lane) * 4, cnt[i], q.size, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < V; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) s += v[i][k];
-  const float m = sum_lanes<L>(s, sh[0]) * q.inv_d;
+  const float m = sum_lanes<L>(s, sh[0]) / q.d;
   s = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i)
@@ -304,8 +358,8 @@ __global__ __launch_bounds__(256) void gn_fwd_rows_kernel(NormGeom q, const floa
     }
     if (cnt[i] > 0) {
       float ga[4] = {1.0f, 1.0f, 1.0f, 1.0f}, be[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4];
-      if (gamma) SrcF::load4(gamma, c0 + (i * L + lane) * 4, cnt[i], ga);
-      if (beta) SrcF::load4(beta, c0 + (i * L + lane) * 4, cnt[i], be);
+      if (gamma) load4<MODE>(gamma, c0 + (i * L + lane) * 4, cnt[i], q.C, ga);
+      if (beta) load4<MODE>(beta, c0 + (i * L + lane) * 4, cnt[i], q.C, be);
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[k] = (v[i][k] - m) * r * ga[k] + be[k];
       act4(q.silu, q.slope, o);
@@ -317,7 +371,7 @@ __global__ __launch_bounds__(256) void gn_fwd_rows_kernel(NormGeom q, const floa
 // A workgroup stays with one group of channels and walks over a chunk of the rows, so a lane's channels are fixed: gamma,
 // beta and the channel sums stay in registers, and the sums cross lanes once per workgroup.
 // part (or null): [2][chunks][C].
-template <int L, int V, class SRC>
+template <int L, int V, int MODE, class SRC>
 __global__ __launch_bounds__(256) void gn_bwd_rows_kernel(NormGeom q, int chunks, SRC x, const float* gamma, const float* beta,
                                                           const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx,
                                                           float* part) {
@@ -337,8 +391,8 @@ __global__ __launch_bounds__(256) void gn_bwd_rows_kernel(NormGeom q, int chunks
       ga[i][k] = 1.0f;
       be[i][k] = sa[i][k] = sb[i][k] = 0.0f;
     }
-    if (gamma) SrcF::load4(gamma, c0 + (i * L + lane) * 4, cnt[i], ga[i]);
-    if (beta) SrcF::load4(beta, c0 + (i * L + lane) * 4, cnt[i], be[i]);
+    if (gamma) load4<MODE>(gamma, c0 + (i * L + lane) * 4, cnt[i], q.C, ga[i]);
+    if (beta) load4<MODE>(beta, c0 + (i * L + lane) * 4, cnt[i], q.C, be[i]);
   }
   for (int nn = n0; nn < n1; nn += S) {   // all lanes together: the row sums may cross wavefronts
     const int n = nn + (int)slot;
@@ -348,8 +402,8 @@ __global__ __launch_bounds__(256) void gn_bwd_rows_kernel(NormGeom q, int chunks
     float xh[V][4], dp[V][4], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      x.load(base + (i * L + lane) * 4, in ? cnt[i] : 0, xh[i]);
-      SrcF::load4(dy, base + (i * L + lane) * 4, in ? cnt[i] : 0, dp[i]);
+      x.template load<MODE>(base + (i * L + lane) * 4, in ? cnt[i] : 0, q.size, xh[i]);
+      load4<MODE>(dy, base + (i * L + lane) * 4, in ? cnt[i] : 0, q.size, dp[i]);
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -379,7 +433,7 @@ __global__ __launch_bounds__(256) void gn_bwd_rows_kernel(NormGeom q, int chunks
       const int c = in ? cnt[i] : 0;
       if (c > 0) {
         float o[4];
-        if (beta_dx) SrcF::load4(dx, at, c, o);
+        if (beta_dx) load4<MODE>(dx, at, c, q.size, o);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float e = r * (dp[i][k] - s1 - xh[i][k] * s2);
@@ -414,10 +468,111 @@ __global__ __launch_bounds__(256) void gn_bwd_rows_kernel(NormGeom q, int chunks
   }
 }
 
+// ---- channels last, small problems ------------------------------------------------------------------------------------
+//
+// One workgroup per row again, element by element: a lane keeps one channel of the group and every PT-th pixel.  The row's
+// pieces of Cg floats make poor use of memory lines, but one launch does it: for tensors up to a megaelement, which the
+// caches hold, three launches (three more backward) take longer than their lines (3 x 37 x 41 x 60, step: 25 -> 20 us).
+template <int T, int V>
+__global__ __launch_bounds__(T) void gn_fwd_gather_kernel(NormGeom q, int pt, const float* x, const float* gamma, const float* beta, float* y,
+                                                          float* mean, float* rstd) {
+  __shared__ float sh[2][T / 64];
+  const uint32_t row = blockIdx.x, n = row / q.G, g = row % q.G;
+  const int pl = threadIdx.x / q.Cg, c = g * q.Cg + ((int)threadIdx.x - pl * q.Cg);
+  const int p0 = pl < pt ? pl : q.HW;   // lanes behind the last whole set of channels have no pixels
+  float v[V], s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = x[(n * q.HW + min(p0 + i * pt, q.HW - 1)) * q.C + c];
+  const float ga = gamma ? gamma[c] : 1.0f, be = beta ? beta[c] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) s += p0 + i * pt < q.HW ? v[i] : 0.0f;
+  const float m = sum_all<T>(s, sh[0]) / q.d;
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float d = p0 + i * pt < q.HW ? v[i] - m : 0.0f;
+    s += d * d;
+  }
+  const float r = 1.0f / sqrtf(sum_all<T>(s, sh[1]) * q.inv_d + q.eps);
+  if (threadIdx.x == 0) {
+    mean[row] = m;
+    rstd[row] = r;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (p0 + i * pt < q.HW) {
+      const float p = (v[i] - m) * r * ga + be;
+      y[(n * q.HW + p0 + i * pt) * q.C + c] = q.silu ? p * sigmoid(p) : p >= 0.0f ? p : q.slope * p;
+    }
+  }
+}
+
+template <int T, int V, class SRC>
+__global__ __launch_bounds__(T) void gn_bwd_gather_kernel(NormGeom q, int pt, SRC x, const float* gamma, const float* beta, const float* mean,
+                                                          const float* rstd, const float* dy, float* dx, int beta_dx, float* part) {
+  __shared__ float sh[2][T / 64], ch[2][T];
+  const uint32_t row = blockIdx.x, n = row / q.G, g = row % q.G;
+  const int pl = threadIdx.x / q.Cg, c = g * q.Cg + ((int)threadIdx.x - pl * q.Cg);
+  const int p0 = pl < pt ? pl : q.HW;
+  const float m = mean[row], r = rstd[row];
+  float v[V], d[V], a = 0.0f, b = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t at = (n * q.HW + min(p0 + i * pt, q.HW - 1)) * q.C + c;
+    v[i] = x.at(at);
+    d[i] = dy[at];
+  }
+  const float ga = gamma ? gamma[c] : 1.0f, be = beta ? beta[c] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const bool in = p0 + i * pt < q.HW;
+    v[i] = (v[i] - m) * r;
+    const float p = v[i] * ga + be;
+    if (q.silu) {
+      const float s = sigmoid(p);
+      d[i] *= fmaf(p * s, 1.0f - s, s);
+    } else {
+      d[i] = p >= 0.0f ? d[i] : q.slope * d[i];
+    }
+    a += in ? d[i] : 0.0f;
+    b += in ? d[i] * v[i] : 0.0f;
+  }
+  if (part) {   // over the pixel lanes of a channel, in halves
+    ch[0][threadIdx.x] = a;
+    ch[1][threadIdx.x] = b;
+    for (int h = pt; h > 1;) {
+      const int half = (h + 1) >> 1;
+      __syncthreads();
+      if (pl + half < h) {
+        ch[0][threadIdx.x] += ch[0][threadIdx.x + half * q.Cg];
+        ch[1][threadIdx.x] += ch[1][threadIdx.x + half * q.Cg];
+      }
+      h = half;
+    }
+    if (pl == 0) {
+      part[n * q.C + c] = ch[0][threadIdx.x];
+      part[(uint32_t)(q.N + n) * q.C + c] = ch[1][threadIdx.x];
+    }
+  }
+  if (!dx) return;
+  const float s1 = sum_all<T>(a * ga, sh[0]) * q.inv_d, s2 = sum_all<T>(b * ga, sh[1]) * q.inv_d;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (p0 + i * pt < q.HW) {
+      float* o = dx + (n * q.HW + p0 + i * pt) * q.C + c;
+      const float e = r * (d[i] * ga - s1 - v[i] * s2);
+      *o = beta_dx ? *o + e : e;
+    }
+  }
+}
+
 // ---- rows too long for registers, and channels last -----------------------------------------------------------------
 //
-// Three launches: sums per channel and chunk of pixels, the rows' statistics from them, the result.  x is read twice;
-// the host takes as many images at a time as stay in the memory-side cache between the two reads.
+// Three launches: sums per channel and chunk of pixels, the rows' statistics from them, the result.  x is read twice; the
+// second time from its end backwards, where what the first reading left in the 256 MB memory-side cache still is.
+// Taking the images in batches that fit that cache was slower (16 x 128 x 128 x 256 forward: 276 us in batches of 96 MB, 208 of
+// 160 MB, 166 in one): the cache saves less than each batch's three short launches cost.
+// 16 x 128 x 128 x 256 forward 160 us = 805 MB at 5.0 TB/s; 8 x 64 x 64 x 320 step from 8 bits 87 us.
 //
 // Means and sums of squared distances of two sets join as
 //   n = na + nb, d = mb - ma:  m = ma + d nb / n,  M = Ma + Mb + d^2 na nb / n
@@ -427,7 +582,7 @@ struct Stat {
 __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
   const float n = a.n + b.n;
   if (n == 0.0f) return a;
-  const float f = b.n / n, d = b.m - a.m;
+  const float f = b.n * __builtin_amdgcn_rcpf(n), d = b.m - a.m;
   // an empty side has weight 0 however far its m is: the weight goes in before the square
   return {n, a.m + d * f, a.M + b.M + d * (d * (a.n * f))};
 }
@@ -439,8 +594,9 @@ struct PlanePos {
   int count;   // pixels of this wavefront's chunk
   bool in;
 };
-__device__ __forceinline__ PlanePos plane_pos(const NormGeom& q, int chunks) {
-  const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 6);
+// back: last image first
+__device__ __forceinline__ PlanePos plane_pos(const NormGeom& q, int chunks, bool back) {
+  const uint32_t w = (back ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * 4 + (threadIdx.x >> 6);
   PlanePos p;
   p.in = w < (uint32_t)q.nb * q.C * chunks;
   const uint32_t plane = w / chunks;
@@ -452,19 +608,19 @@ __device__ __forceinline__ PlanePos plane_pos(const NormGeom& q, int chunks) {
   return p;
 }
 
+template <int MODE>
 __global__ __launch_bounds__(256) void gn_stats_first_kernel(NormGeom q, int chunks, const float* x, float2* part) {
-  const PlanePos p = plane_pos(q, chunks);
+  const PlanePos p = plane_pos(q, chunks, false);
   if (!p.in) return;
   const int lane = threadIdx.x & 63;
   float v[16][4], s = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (i * 256 < p.count) SrcF::load4(x, p.base + i * 256 + lane * 4, min(max(p.count - i * 256 - lane * 4, 0), 4), v[i]);
+    load4<MODE>(x, p.base + i * 256 + lane * 4, min(max(p.count - i * 256 - lane * 4, 0), 4), q.size, v[i]);
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (i * 256 < p.count)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s += v[i][k];
+    for (int k = 0; k < 4; ++k) s += v[i][k];
   const float m = sum_all<64>(s, nullptr) / (float)p.count;
   s = 0.0f;
 #pragma unroll
@@ -479,11 +635,11 @@ __global__ __launch_bounds__(256) void gn_stats_first_kernel(NormGeom q, int chu
   if (lane == 0) part[((p.n - q.n0) * chunks + p.chunk) * q.C + p.c] = make_float2(m, s);
 }
 
-template <bool KEEP>
+template <int MODE, bool KEEP>
 __global__ __launch_bounds__(256) void gn_apply_first_kernel(NormGeom q, int chunks, const float* x, const float* gamma, const float* beta,
                                                              const float* mean, const float* rstd, float* y, uint8_t* codes,
                                                              uint8_t* bytes) {
-  const PlanePos p = plane_pos(q, chunks);
+  const PlanePos p = plane_pos(q, chunks, true);
   if (!p.in) return;
   const int lane = threadIdx.x & 63;
   const uint32_t row = p.n * q.G + p.c / q.Cg;
@@ -494,7 +650,7 @@ __global__ __launch_bounds__(256) void gn_apply_first_kernel(NormGeom q, int chu
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       cnt[j] = min(max(p.count - i0 - j * 256 - lane * 4, 0), 4);
-      SrcF::load4(x, p.base + i0 + j * 256 + lane * 4, cnt[j], v[j]);
+      load4<MODE>(x, p.base + i0 + j * 256 + lane * 4, cnt[j], q.size, v[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -515,31 +671,37 @@ __global__ __launch_bounds__(256) void gn_apply_first_kernel(NormGeom q, int chu
   }
 }
 
-template <class SRC>
+template <int MODE, class SRC>
 __global__ __launch_bounds__(256) void gn_sums_first_kernel(NormGeom q, int chunks, SRC x, const float* gamma, const float* beta,
                                                             const float* mean, const float* rstd, const float* dy, float* pa, float* pb) {
-  const PlanePos p = plane_pos(q, chunks);
+  const PlanePos p = plane_pos(q, chunks, false);
   if (!p.in) return;
   const int lane = threadIdx.x & 63;
   const uint32_t row = p.n * q.G + p.c / q.Cg;
   const float m = mean[row], r = rstd[row], ga = gamma ? gamma[p.c] : 1.0f, be = beta ? beta[p.c] : 0.0f;
   float a = 0.0f, b = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < p.count; i += 256) {
-    const int cnt = min(max(p.count - i - lane * 4, 0), 4);
-    float v[4], d[4], pre[4];
-    x.load(p.base + i + lane * 4, cnt, v);
-    SrcF::load4(dy, p.base + i + lane * 4, cnt, d);
+  for (int i0 = 0; i0 < p.count; i0 += 1024) {   // four groups in flight
+    float v[4][4], d[4][4], pre[4];
+    int cnt[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = k < cnt ? (v[k] - m) * r : 0.0f;
-      pre[k] = v[k] * ga + be;
+    for (int j = 0; j < 4; ++j) {
+      cnt[j] = min(max(p.count - i0 - j * 256 - lane * 4, 0), 4);
+      x.template load<MODE>(p.base + i0 + j * 256 + lane * 4, cnt[j], q.size, v[j]);
+      load4<MODE>(dy, p.base + i0 + j * 256 + lane * 4, cnt[j], q.size, d[j]);
     }
-    slope4(q.silu, q.slope, pre, d);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      a += d[k];
-      b += d[k] * v[k];
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[j][k] = k < cnt[j] ? (v[j][k] - m) * r : 0.0f;
+        pre[k] = v[j][k] * ga + be;
+      }
+      slope4(q.silu, q.slope, pre, d[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        a += d[j][k];
+        b += d[j][k] * v[j][k];
+      }
     }
   }
   a = sum_all<64>(a, nullptr);
@@ -551,36 +713,43 @@ __global__ __launch_bounds__(256) void gn_sums_first_kernel(NormGeom q, int chun
   }
 }
 
-template <class SRC>
+template <int MODE, class SRC>
 __global__ __launch_bounds__(256) void gn_dx_first_kernel(NormGeom q, int chunks, SRC x, const float* gamma, const float* beta,
                                                           const float* mean, const float* rstd, const float* dy, const float2* s12,
                                                           float* dx, int beta_dx) {
-  const PlanePos p = plane_pos(q, chunks);
+  const PlanePos p = plane_pos(q, chunks, true);
   if (!p.in) return;
   const int lane = threadIdx.x & 63;
   const uint32_t row = p.n * q.G + p.c / q.Cg;
   const float m = mean[row], r = rstd[row], ga = gamma ? gamma[p.c] : 1.0f, be = beta ? beta[p.c] : 0.0f;
   const float2 s = s12[row];
-#pragma unroll 4
-  for (int i = 0; i < p.count; i += 256) {
-    const int cnt = min(max(p.count - i - lane * 4, 0), 4);
-    const uint32_t at = p.base + i + lane * 4;
-    float v[4], d[4], pre[4], o[4];
-    x.load(at, cnt, v);
-    SrcF::load4(dy, at, cnt, d);
-    if (beta_dx) SrcF::load4(dx, at, cnt, o);
+  for (int i0 = 0; i0 < p.count; i0 += 1024) {
+    float v[4][4], d[4][4], pre[4];
+    int cnt[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = (v[k] - m) * r;
-      pre[k] = v[k] * ga + be;
+    for (int j = 0; j < 4; ++j) {
+      cnt[j] = min(max(p.count - i0 - j * 256 - lane * 4, 0), 4);
+      x.template load<MODE>(p.base + i0 + j * 256 + lane * 4, cnt[j], q.size, v[j]);
+      load4<MODE>(dy, p.base + i0 + j * 256 + lane * 4, cnt[j], q.size, d[j]);
     }
-    slope4(q.silu, q.slope, pre, d);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float e = r * (d[k] * ga - s.x - v[k] * s.y);
-      o[k] = beta_dx ? o[k] + e : e;
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = p.base + i0 + j * 256 + lane * 4;
+      float o[4];
+      if (beta_dx) load4<MODE>(dx, at, cnt[j], q.size, o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[j][k] = (v[j][k] - m) * r;
+        pre[k] = v[j][k] * ga + be;
+      }
+      slope4(q.silu, q.slope, pre, d[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float e = r * (d[j][k] * ga - s.x - v[j][k] * s.y);
+        o[k] = beta_dx ? o[k] + e : e;
+      }
+      store4(dx, at, cnt[j], o);
     }
-    store4(dx, at, cnt, o);
   }
 }
 
@@ -593,9 +762,9 @@ struct LastPos {
   uint32_t n, c, chunk;
   int x, y, p0, p1, cnt;   // lane's place; pixels; channels of this lane that exist (0: none)
 };
-__device__ __forceinline__ LastPos last_pos(const NormGeom& q, const LastTile& t) {
+__device__ __forceinline__ LastPos last_pos(const NormGeom& q, const LastTile& t, bool back) {
   LastPos p;
-  const uint32_t slab = blockIdx.x % t.slabs, k = blockIdx.x / t.slabs;
+  const uint32_t w = back ? gridDim.x - 1 - blockIdx.x : blockIdx.x, slab = w % t.slabs, k = w / t.slabs;
   p.chunk = k % t.chunks;
   p.n = q.n0 + k / t.chunks;
   p.y = threadIdx.x / t.tx;
@@ -607,9 +776,10 @@ __device__ __forceinline__ LastPos last_pos(const NormGeom& q, const LastTile& t
   return p;
 }
 
+template <int MODE>
 __global__ __launch_bounds__(256) void gn_stats_last_kernel(NormGeom q, LastTile t, const float* x, float2* part) {
   __shared__ float sm[4][256], sM[4][256], sn[256];
-  const LastPos p = last_pos(q, t);
+  const LastPos p = last_pos(q, t, false);
   constexpr int B = 8;
   Stat st[4] = {};
   if (p.cnt > 0) {
@@ -621,9 +791,9 @@ __global__ __launch_bounds__(256) void gn_stats_last_kernel(NormGeom q, LastTile
         const int pix = q0 + i * t.ty;
         const bool in = pix < p.p1;
         nv += in;
-        SrcF::load4(x, (p.n * q.HW + pix) * q.C + p.c, in ? p.cnt : 0, v[i]);
+        load4<MODE>(x, (p.n * q.HW + pix) * q.C + p.c, in ? p.cnt : 0, q.size, v[i]);
       }
-      const float inv = 1.0f / (float)nv;
+      const float inv = __builtin_amdgcn_rcpf((float)nv);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float s = 0.0f, M = 0.0f;
@@ -670,23 +840,27 @@ __global__ __launch_bounds__(256) void gn_stats_last_kernel(NormGeom q, LastTile
 
 // Statistics of row (n, g) from those of its channels and chunks of `pix` pixels.
 __global__ __launch_bounds__(256) void gn_finish_kernel(NormGeom q, int chunks, int pix, const float2* part, float* mean, float* rstd) {
-  __shared__ Stat sh[256];
+  __shared__ Stat sh[4];
   const uint32_t n = blockIdx.x / q.G, g = blockIdx.x % q.G;   // n: image of the batch
   Stat s = {0.0f, 0.0f, 0.0f};
+#pragma unroll 4
   for (int j = threadIdx.x; j < chunks * q.Cg; j += 256) {
     const int chunk = j / q.Cg, c = j - chunk * q.Cg;
     const float2 e = part[(n * chunks + chunk) * q.C + g * q.Cg + c];
     s = join(s, Stat{(float)min(pix, q.HW - chunk * pix), e.x, e.y});
   }
-  sh[threadIdx.x] = s;
-  for (int w = 128; w > 0; w >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < w) sh[threadIdx.x] = join(sh[threadIdx.x], sh[threadIdx.x + w]);
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) {
+    const Stat o = {__shfl_down(s.n, w, 64), __shfl_down(s.m, w, 64), __shfl_down(s.M, w, 64)};
+    s = join(s, o);   // lane 0's tree is the only one that counts
   }
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    s = join(join(sh[0], sh[1]), join(sh[2], sh[3]));
     const uint32_t row = (q.n0 + n) * q.G + g;
-    mean[row] = sh[0].m;
-    rstd[row] = 1.0f / sqrtf(sh[0].M * q.inv_d + q.eps);
+    mean[row] = s.m;
+    rstd[row] = 1.0f / sqrtf(s.M * q.inv_d + q.eps);
   }
 }
 
@@ -696,21 +870,30 @@ struct LaneRows {
 };
 __device__ __forceinline__ void lane_rows(const NormGeom& q, const LastPos& p, const float* gamma, const float* beta, const float* mean,
                                           const float* rstd, LaneRows* l) {
+  uint32_t c[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const bool in = k < p.cnt;
-    const uint32_t c = in ? p.c + k : 0, row = p.n * q.G + c / q.Cg;
-    l->m[k] = in ? mean[row] : 0.0f;
-    l->r[k] = in ? rstd[row] : 0.0f;
-    l->ga[k] = gamma ? gamma[c] : 1.0f;
-    l->be[k] = beta ? beta[c] : 0.0f;
+    c[k] = k < p.cnt ? p.c + k : 0;
+    const uint32_t row = p.n * q.G + c[k] / q.Cg;
+    l->m[k] = mean[row];
+    l->r[k] = rstd[row];
+    l->ga[k] = 1.0f;
+    l->be[k] = 0.0f;
+  }
+  if (gamma) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) l->ga[k] = gamma[c[k]];
+  }
+  if (beta) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) l->be[k] = beta[c[k]];
   }
 }
 
-template <bool KEEP>
+template <int MODE, bool KEEP>
 __global__ __launch_bounds__(256) void gn_apply_last_kernel(NormGeom q, LastTile t, const float* x, const float* gamma, const float* beta,
                                                             const float* mean, const float* rstd, float* y, uint8_t* codes, uint8_t* bytes) {
-  const LastPos p = last_pos(q, t);
+  const LastPos p = last_pos(q, t, true);
   LaneRows l;
   lane_rows(q, p, gamma, beta, mean, rstd, &l);
   for (int pix0 = p.p0 + p.y; pix0 < p.p1; pix0 += 4 * t.ty) {   // four loads in flight
@@ -720,7 +903,7 @@ __global__ __launch_bounds__(256) void gn_apply_last_kernel(NormGeom q, LastTile
     for (int j = 0; j < 4; ++j) {
       const int pix = pix0 + j * t.ty;
       cnt[j] = pix < p.p1 ? p.cnt : 0;
-      SrcF::load4(x, (p.n * q.HW + pix) * q.C + p.c, cnt[j], v[j]);
+      load4<MODE>(x, (p.n * q.HW + pix) * q.C + p.c, cnt[j], q.size, v[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -741,30 +924,35 @@ __global__ __launch_bounds__(256) void gn_apply_last_kernel(NormGeom q, LastTile
   }
 }
 
-template <class SRC>
+template <int MODE, class SRC>
 __global__ __launch_bounds__(256) void gn_sums_last_kernel(NormGeom q, LastTile t, SRC x, const float* gamma, const float* beta,
                                                            const float* mean, const float* rstd, const float* dy, float* pa, float* pb) {
   __shared__ float sh[8][256];
-  const LastPos p = last_pos(q, t);
+  const LastPos p = last_pos(q, t, false);
   LaneRows l;
   lane_rows(q, p, gamma, beta, mean, rstd, &l);
   float a[4] = {}, b[4] = {};
-#pragma unroll 4
-  for (int pix = p.p0 + p.y; pix < p.p1; pix += t.ty) {
-    const uint32_t at = (p.n * q.HW + pix) * q.C + p.c;
-    float v[4], d[4], pre[4];
-    x.load(at, p.cnt, v);
-    SrcF::load4(dy, at, p.cnt, d);
+  for (int pix0 = p.p0 + p.y; pix0 < p.p1; pix0 += 4 * t.ty) {   // four pixels in flight
+    float v[4][4], d[4][4], pre[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = (v[k] - l.m[k]) * l.r[k];
-      pre[k] = v[k] * l.ga[k] + l.be[k];
+    for (int j = 0; j < 4; ++j) {
+      const int pix = pix0 + j * t.ty, cnt = pix < p.p1 ? p.cnt : 0;
+      x.template load<MODE>((p.n * q.HW + pix) * q.C + p.c, cnt, q.size, v[j]);
+      load4<MODE>(dy, (p.n * q.HW + pix) * q.C + p.c, cnt, q.size, d[j]);   // 0 where there is no pixel
     }
-    slope4(q.silu, q.slope, pre, d);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      a[k] += d[k];
-      b[k] += d[k] * v[k];
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[j][k] = (v[j][k] - l.m[k]) * l.r[k];
+        pre[k] = v[j][k] * l.ga[k] + l.be[k];
+      }
+      slope4(q.silu, q.slope, pre, d[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        a[k] += d[j][k];
+        b[k] += d[j][k] * v[j][k];
+      }
     }
   }
 #pragma unroll
@@ -792,11 +980,11 @@ __global__ __launch_bounds__(256) void gn_sums_last_kernel(NormGeom q, LastTile 
   }
 }
 
-template <class SRC>
+template <int MODE, class SRC>
 __global__ __launch_bounds__(256) void gn_dx_last_kernel(NormGeom q, LastTile t, SRC x, const float* gamma, const float* beta,
                                                          const float* mean, const float* rstd, const float* dy, const float2* s12,
                                                          float* dx, int beta_dx) {
-  const LastPos p = last_pos(q, t);
+  const LastPos p = last_pos(q, t, true);
   LaneRows l;
   lane_rows(q, p, gamma, beta, mean, rstd, &l);
   float s1[4], s2[4];
@@ -806,53 +994,43 @@ __global__ __launch_bounds__(256) void gn_dx_last_kernel(NormGeom q, LastTile t,
     s1[k] = s.x;
     s2[k] = s.y;
   }
-#pragma unroll 4
-  for (int pix = p.p0 + p.y; pix < p.p1; pix += t.ty) {
-    const uint32_t at = (p.n * q.HW + pix) * q.C + p.c;
-    float v[4], d[4], pre[4], o[4];
-    x.load(at, p.cnt, v);
-    SrcF::load4(dy, at, p.cnt, d);
-    if (beta_dx) SrcF::load4(dx, at, p.cnt, o);
+  for (int pix0 = p.p0 + p.y; pix0 < p.p1; pix0 += 4 * t.ty) {
+    float v[4][4], d[4][4], pre[4];
+    int cnt[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = (v[k] - l.m[k]) * l.r[k];
-      pre[k] = v[k] * l.ga[k] + l.be[k];
+    for (int j = 0; j < 4; ++j) {
+      const int pix = pix0 + j * t.ty;
+      cnt[j] = pix < p.p1 ? p.cnt : 0;
+      x.template load<MODE>((p.n * q.HW + pix) * q.C + p.c, cnt[j], q.size, v[j]);
+      load4<MODE>(dy, (p.n * q.HW + pix) * q.C + p.c, cnt[j], q.size, d[j]);
     }
-    slope4(q.silu, q.slope, pre, d);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float e = l.r[k] * (d[k] * l.ga[k] - s1[k] - v[k] * s2[k]);
-      o[k] = beta_dx ? o[k] + e : e;
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = (p.n * q.HW + pix0 + j * t.ty) * q.C + p.c;
+      float o[4];
+      if (beta_dx) load4<MODE>(dx, at, cnt[j], q.size, o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[j][k] = (v[j][k] - l.m[k]) * l.r[k];
+        pre[k] = v[j][k] * l.ga[k] + l.be[k];
+      }
+      slope4(q.silu, q.slope, pre, d[j]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float e = l.r[k] * (d[j][k] * l.ga[k] - s1[k] - v[j][k] * s2[k]);
+        o[k] = beta_dx ? o[k] + e : e;
+      }
+      store4(dx, at, cnt[j], o);
     }
-    store4(dx, at, p.cnt, o);
   }
 }
 
-// row (n, g): s1 and s2 from the sums of its channels and chunks
-__global__ __launch_bounds__(256) void gn_finish_dx_kernel(NormGeom q, int chunks, const float* gamma, const float* pa, const float* pb,
-                                                           float2* s12) {
-  __shared__ float sh[2][4];
-  const uint32_t n = q.n0 + blockIdx.x / q.G, g = blockIdx.x % q.G;
-  float a = 0.0f, b = 0.0f;
-  for (int j = threadIdx.x; j < chunks * q.Cg; j += 256) {
-    const int chunk = j / q.Cg, c = g * q.Cg + (j - chunk * q.Cg);
-    const float ga = gamma ? gamma[c] : 1.0f;
-    a += ga * pa[(n * chunks + chunk) * q.C + c];
-    b += ga * pb[(n * chunks + chunk) * q.C + c];
-  }
-  a = sum_all<256>(a, sh[0]);
-  b = sum_all<256>(b, sh[1]);
-  if (threadIdx.x == 0) s12[n * q.G + g] = make_float2(a * q.inv_d, b * q.inv_d);
-}
-
-// dbeta, dgamma: column sums of the K rows of pa and pb.  A workgroup takes 32 channels and the rows [y per, (y + 1) per):
-// 8 lanes per channel walk over them, then add up in order.  With gridDim.y > 1 the sums are left as rows of outa / outb
-// for a second launch.
-__global__ __launch_bounds__(256) void gn_params_kernel(int K, int per, int C, const float* pa, const float* pb, float* outa, int beta_a,
-                                                        float* outb, int beta_b) {
+// Column sums of the K rows of pa and pb: a workgroup takes 32 channels and the rows [k0, k1), 8 lanes per channel walk over
+// them, then add up in order.
+__device__ __forceinline__ void column_sums(uint32_t block, int k0, int k1, int C, const float* pa, const float* pb, float* outa, int beta_a,
+                                            float* outb, int beta_b) {
   __shared__ float sh[2][8][33];
-  const int li = threadIdx.x & 31, lk = threadIdx.x >> 5, c = blockIdx.x * 32 + li;
-  const int k0 = blockIdx.y * per, k1 = min(k0 + per, K);
+  const int li = threadIdx.x & 31, lk = threadIdx.x >> 5, c = block * 32 + li;
   float a = 0.0f, b = 0.0f;
   if (c < C) {
 #pragma unroll 4
@@ -870,10 +1048,40 @@ __global__ __launch_bounds__(256) void gn_params_kernel(int K, int per, int C, c
       a += sh[0][k][li];
       b += sh[1][k][li];
     }
-    const uint32_t at = blockIdx.y * (uint32_t)C + c;
-    if (outa) outa[at] = beta_a ? outa[at] + a : a;
-    if (outb) outb[at] = beta_b ? outb[at] + b : b;
+    if (outa) outa[c] = beta_a ? outa[c] + a : a;
+    if (outb) outb[c] = beta_b ? outb[c] + b : b;
   }
+}
+
+// row (n, g): s1 and s2 from the sums of its channels and chunks.  Workgroups behind the rows form dbeta and dgamma from the
+// K rows of the same sums, in the launch that is there anyway.
+__global__ __launch_bounds__(256) void gn_finish_dx_kernel(NormGeom q, int chunks, const float* gamma, const float* pa, const float* pb,
+                                                           float2* s12, int K, float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta) {
+  __shared__ float sh[2][4];
+  const uint32_t rows = (uint32_t)q.nb * q.G;
+  if (blockIdx.x >= rows) {
+    column_sums(blockIdx.x - rows, 0, K, q.C, pa, pb, dbeta, beta_dbeta, dgamma, beta_dgamma);
+    return;
+  }
+  const uint32_t n = q.n0 + blockIdx.x / q.G, g = blockIdx.x % q.G;
+  float a = 0.0f, b = 0.0f;
+  for (int j = threadIdx.x; j < chunks * q.Cg; j += 256) {
+    const int chunk = j / q.Cg, c = g * q.Cg + (j - chunk * q.Cg);
+    const float ga = gamma ? gamma[c] : 1.0f;
+    a += ga * pa[(n * chunks + chunk) * q.C + c];
+    b += ga * pb[(n * chunks + chunk) * q.C + c];
+  }
+  a = sum_all<256>(a, sh[0]);
+  b = sum_all<256>(b, sh[1]);
+  if (threadIdx.x == 0) s12[n * q.G + g] = make_float2(a * q.inv_d, b * q.inv_d);
+}
+
+// dbeta, dgamma; with gridDim.y > 1 the sums over `per` rows each, left as rows of outa / outb for a second launch
+__global__ __launch_bounds__(256) void gn_params_kernel(int K, int per, int C, const float* pa, const float* pb, float* outa, int beta_a,
+                                                        float* outb, int beta_b) {
+  const int k0 = blockIdx.y * per;
+  const uint64_t at = (uint64_t)blockIdx.y * C;
+  column_sums(blockIdx.x, k0, min(k0 + per, K), C, pa, pb, outa ? outa + at : nullptr, beta_a, outb ? outb + at : nullptr, beta_b);
 }
 
 int launch_encode8(DeviceCtx*, uint64_t, const float*, void*);
@@ -893,14 +1101,16 @@ static int make_geom(const lnn_group_norm_desc* d, NormGeom* q) {
   q->HW = d->HW;
   q->G = d->groups;
   q->Cg = d->C / d->groups;
-  q->last = d->channels_last != 0 || d->HW == 1;   // with one pixel the two layouts are one
+  q->last = (d->channels_last != 0 && d->C > 1) || d->HW == 1;   // with one channel or one pixel the two layouts are one
   q->n0 = 0;
   q->nb = d->N;
   q->silu = d->act == LNN_ACT_SILU;
   q->slope = d->act == LNN_ACT_NONE ? 1.0f : d->slope;
   q->eps = d->eps;
   q->row0 = 0;
+  q->size = (uint32_t)((uint64_t)d->N * d->C * d->HW);
   q->D = (uint32_t)q->Cg * (uint32_t)q->HW;
+  q->d = (float)q->D;
   q->inv_d = (float)(1.0 / (double)q->D);
   return LNN_OK;
 }
@@ -910,20 +1120,25 @@ struct ResPlan {
   Units un;
   int T, V;
 };
-static bool res_plan(const DeviceCtx* ctx, const NormGeom& q, int most, ResPlan* p) {
+// most: groups per lane at 1024 lanes; most512: the same at 512
+static bool res_plan(const NormGeom& q, int most, int most512, ResPlan* p) {
   if (q.last) return false;
   // the shortest unit that holds a plane, or whole wavefronts
   p->un.ul = q.HW <= 4 ? 0 : q.HW <= 16 ? 2 : q.HW <= 64 ? 4 : 6;
   p->un.per = ((q.HW + 3) / 4 + (1 << p->un.ul) - 1) >> p->un.ul;
   const uint64_t lanes = ((uint64_t)q.Cg * p->un.per) << p->un.ul;
   p->un.total = q.Cg * p->un.per;
-  if (lanes > 1024u * most || p->un.total > 7000) return false;   // 7000: the backward pass keeps two sums per unit in 64 KB
+  if (lanes > 1024u * most || p->un.total > 3500) return false;   // 3500: two sums per unit, gamma and beta in 64 KB of LDS
   p->un.dper = make_fastdiv((uint32_t)p->un.per);
-  p->T = lanes <= 64 ? 64 : lanes <= 256u * most ? 256 : 1024;
-  if (p->T == 256 && lanes >= 1024 && q.N * q.G <= 2 * ctx->cus) p->T = 1024;
-  const uint64_t v = (lanes + p->T - 1) / p->T;
-  p->V = v <= 1 ? 1 : v <= 2 ? 2 : v <= 4 ? 4 : v <= 8 ? 8 : 16;
-  return true;
+  p->T = lanes <= 64 ? 64 : lanes <= 1024 ? 256 : lanes <= 512u * most512 ? 512 : 1024;
+  if (lanes > 1024 && q.N * q.G <= 256) p->T = 1024;   // fewer rows than compute units: more lanes to each
+  static const int sizes[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 13, 16};
+  for (int v : sizes)
+    if (lanes <= (uint64_t)p->T * v) {
+      p->V = v;
+      return true;
+    }
+  return false;
 }
 
 constexpr uint32_t kMaxRows = 1u << 21;   // of one launch
@@ -933,10 +1148,10 @@ static void fwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const fl
                     float* mean, float* rstd, uint8_t* codes, uint8_t* bytes) {
   const unsigned rows = (unsigned)(q.N * q.G) - q.row0 < kMaxRows ? (unsigned)(q.N * q.G) - q.row0 : kMaxRows;
   if (codes)
-    hipLaunchKernelGGL((gn_fwd_res_kernel<T, V, true>), dim3(rows), dim3(T), 0, ctx->stream, q, un, x, gamma, beta, y,
+    hipLaunchKernelGGL((gn_fwd_res_kernel<T, V, G4, true>), dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
                        mean, rstd, codes, bytes);
   else
-    hipLaunchKernelGGL((gn_fwd_res_kernel<T, V, false>), dim3(rows), dim3(T), 0, ctx->stream, q, un, x, gamma, beta, y,
+    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_fwd_res_kernel<T, V, G4, false> : q.size >= 4 ? gn_fwd_res_kernel<T, V, GANY, false> : gn_fwd_res_kernel<T, V, T == 64 ? GTINY : GANY, false>), dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
                        mean, rstd, codes, bytes);
 }
 template <int T, int V>
@@ -944,24 +1159,29 @@ static void bwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const fl
                     const float* gamma, const float* beta, const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx,
                     float* part) {
   const unsigned rows = (unsigned)(q.N * q.G) - q.row0 < kMaxRows ? (unsigned)(q.N * q.G) - q.row0 : kMaxRows;
-  if (codes)
-    hipLaunchKernelGGL((gn_bwd_res_kernel<T, V, Src8>), dim3(rows), dim3(T), (unsigned)un.total * 8, ctx->stream, q, un,
+  if (codes && q.HW % 4 == 0)
+    hipLaunchKernelGGL((gn_bwd_res_kernel<T, V, G4, Src8, Hold8>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
+                       Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
+  else if (codes)
+    hipLaunchKernelGGL((q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, Src8, HoldF> : gn_bwd_res_kernel<T, V, T == 64 ? GTINY : GANY, Src8, HoldF>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
                        Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((gn_bwd_res_kernel<T, V, SrcF>), dim3(rows), dim3(T), (unsigned)un.total * 8, ctx->stream, q, un,
-                       SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
+    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_bwd_res_kernel<T, V, G4, SrcF, HoldF> : q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, SrcF, HoldF> : gn_bwd_res_kernel<T, V, T == 64 ? GTINY : GANY, SrcF, HoldF>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un, SrcF{x}, gamma,
+                       beta, mean, rstd, dy, dx, beta_dx, part);
 }
-#define LNN_RES_CASES(p, F, ...)                                                        \
-  switch ((p).T * 32 + (p).V) {                                                         \
-    case 64 * 32 + 1: F<64, 1>(__VA_ARGS__); break;                                     \
-    case 256 * 32 + 1: F<256, 1>(__VA_ARGS__); break;                                   \
-    case 256 * 32 + 2: F<256, 2>(__VA_ARGS__); break;                                   \
-    case 256 * 32 + 4: F<256, 4>(__VA_ARGS__); break;                                   \
-    case 256 * 32 + 8: F<256, 8>(__VA_ARGS__); break;                                   \
-    case 1024 * 32 + 1: F<1024, 1>(__VA_ARGS__); break;                                 \
-    case 1024 * 32 + 2: F<1024, 2>(__VA_ARGS__); break;                                 \
-    case 1024 * 32 + 4: F<1024, 4>(__VA_ARGS__); break;                                 \
-    case 1024 * 32 + 8: F<1024, 8>(__VA_ARGS__); break;
+#define LNN_RES_CASE(T, V, F, ...) \
+  case T * 32 + V: F<T, V>(__VA_ARGS__); break;
+#define LNN_RES_CASES(p, F, ...)                                                                                   \
+  switch ((p).T * 32 + (p).V) {                                                                                    \
+    LNN_RES_CASE(64, 1, F, __VA_ARGS__)                                                                            \
+    LNN_RES_CASE(256, 1, F, __VA_ARGS__) LNN_RES_CASE(256, 2, F, __VA_ARGS__) LNN_RES_CASE(256, 3, F, __VA_ARGS__) \
+    LNN_RES_CASE(256, 4, F, __VA_ARGS__)                                                                           \
+    LNN_RES_CASE(512, 3, F, __VA_ARGS__) LNN_RES_CASE(512, 4, F, __VA_ARGS__) LNN_RES_CASE(512, 5, F, __VA_ARGS__) \
+    LNN_RES_CASE(512, 6, F, __VA_ARGS__) LNN_RES_CASE(512, 7, F, __VA_ARGS__) LNN_RES_CASE(512, 8, F, __VA_ARGS__) \
+    LNN_RES_CASE(512, 10, F, __VA_ARGS__) LNN_RES_CASE(512, 13, F, __VA_ARGS__)                                    \
+    LNN_RES_CASE(1024, 2, F, __VA_ARGS__) LNN_RES_CASE(1024, 3, F, __VA_ARGS__) LNN_RES_CASE(1024, 4, F, __VA_ARGS__) \
+    LNN_RES_CASE(1024, 5, F, __VA_ARGS__) LNN_RES_CASE(1024, 6, F, __VA_ARGS__) LNN_RES_CASE(1024, 7, F, __VA_ARGS__) \
+    LNN_RES_CASE(1024, 8, F, __VA_ARGS__)
 
 // Lanes per row (L) and groups of four per lane (V) of the kernels for rows of channels alone; L = 0 where a row is longer.
 struct RowPlan {
@@ -997,9 +1217,9 @@ static void fwd_rows(DeviceCtx* ctx, const NormGeom& q, const float* x, const fl
                      float* rstd, uint8_t* codes, uint8_t* bytes) {
   const unsigned blocks = ((unsigned)(q.N * q.G) + 256 / L - 1) / (256 / L);   // a row has at least D / 4 lanes: below 2^24
   if (codes)
-    hipLaunchKernelGGL((gn_fwd_rows_kernel<L, V, true>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
+    hipLaunchKernelGGL((gn_fwd_rows_kernel<L, V, G4, true>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
   else
-    hipLaunchKernelGGL((gn_fwd_rows_kernel<L, V, false>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
+    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_fwd_rows_kernel<L, V, G4, false> : q.C >= 4 ? gn_fwd_rows_kernel<L, V, GANY, false> : gn_fwd_rows_kernel<L, V, L == 4 ? GTINY : GANY, false>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
 }
 template <int L, int V>
 static void bwd_rows(DeviceCtx* ctx, const NormGeom& q, int chunks, const float* x, const uint8_t* codes, const uint8_t* bytes,
@@ -1007,44 +1227,81 @@ static void bwd_rows(DeviceCtx* ctx, const NormGeom& q, int chunks, const float*
                      float* part) {
   const unsigned blocks = (unsigned)chunks * q.G;
   if (codes)
-    hipLaunchKernelGGL((gn_bwd_rows_kernel<L, V, Src8>), dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, Src8{codes, bytes}, gamma, beta,
+    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, Src8> : q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, Src8> : gn_bwd_rows_kernel<L, V, L == 4 ? GTINY : GANY, Src8>), dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, Src8{codes, bytes}, gamma, beta,
                        mean, rstd, dy, dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((gn_bwd_rows_kernel<L, V, SrcF>), dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, SrcF{x}, gamma, beta, mean, rstd,
+    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, SrcF> : q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, SrcF> : gn_bwd_rows_kernel<L, V, L == 4 ? GTINY : GANY, SrcF>), dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, SrcF{x}, gamma, beta, mean, rstd,
                        dy, dx, beta_dx, part);
 }
 
+// Lanes and pixels per lane of the kernels for small channels-last problems; T = 0 where they do not apply.
+struct GatherPlan {
+  int T, V, pt;
+};
+static GatherPlan gather_plan(const NormGeom& q) {
+  GatherPlan p = {0, 0, 0};
+  if (!q.last || q.HW == 1 || q.Cg > 256 || q.size > 1u << 20) return p;
+  for (int T : {256, 1024})
+    for (int V : {1, 4, 8, 16}) {
+      const int pt = T / q.Cg;
+      if (p.T == 0 && (int64_t)pt * V >= q.HW) p = {T, V, pt};
+    }
+  return p;
+}
+#define LNN_GATHER_CASE(T, V, F, ...) \
+  case T * 32 + V: F<T, V>(__VA_ARGS__); break;
+#define LNN_GATHER_CASES(p, F, ...)                                                                                                       \
+  switch ((p).T * 32 + (p).V) {                                                                                                           \
+    LNN_GATHER_CASE(256, 1, F, __VA_ARGS__) LNN_GATHER_CASE(256, 4, F, __VA_ARGS__) LNN_GATHER_CASE(256, 8, F, __VA_ARGS__)               \
+    LNN_GATHER_CASE(256, 16, F, __VA_ARGS__) LNN_GATHER_CASE(1024, 8, F, __VA_ARGS__) LNN_GATHER_CASE(1024, 16, F, __VA_ARGS__)           \
+    default: return set_error(LNN_ERR_INVALID, "group_norm: no kernel for this plan");                                                    \
+  }
+template <int T, int V>
+static void fwd_gather(DeviceCtx* ctx, const NormGeom& q, int pt, const float* x, const float* gamma, const float* beta, float* y, float* mean,
+                       float* rstd) {
+  hipLaunchKernelGGL((gn_fwd_gather_kernel<T, V>), dim3((unsigned)(q.N * q.G)), dim3(T), 0, ctx->stream, q, pt, x, gamma, beta, y, mean, rstd);
+}
+template <int T, int V>
+static void bwd_gather(DeviceCtx* ctx, const NormGeom& q, int pt, const float* x, const uint8_t* codes, const uint8_t* bytes, const float* gamma,
+                       const float* beta, const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx, float* part) {
+  if (codes)
+    hipLaunchKernelGGL((gn_bwd_gather_kernel<T, V, Src8>), dim3((unsigned)(q.N * q.G)), dim3(T), 0, ctx->stream, q, pt, Src8{codes, bytes}, gamma,
+                       beta, mean, rstd, dy, dx, beta_dx, part);
+  else
+    hipLaunchKernelGGL((gn_bwd_gather_kernel<T, V, SrcF>), dim3((unsigned)(q.N * q.G)), dim3(T), 0, ctx->stream, q, pt, SrcF{x}, gamma, beta,
+                       mean, rstd, dy, dx, beta_dx, part);
+}
+
 // The tile of the channels-last kernels, and the chunks of either layout.
-static LastTile last_tile(const DeviceCtx* ctx, const NormGeom& q) {
+static LastTile last_tile(const DeviceCtx* ctx, const NormGeom& q, int images, int most) {
   LastTile t;
   const int cv = (q.C + 3) / 4;
   t.tx = cv < 256 ? cv : 256;
   t.slabs = (cv + 255) / 256;
   t.ty = 256 / t.tx;
-  // a lane walks over 32 pixels, fewer where that leaves the chip short of workgroups
-  int64_t per = 32;
-  while (per > 4 && (int64_t)q.N * t.slabs * ((q.HW + t.ty * per - 1) / (t.ty * per)) < 4 * ctx->cus) per >>= 1;
+  // a lane walks over `most` pixels, fewer where that leaves the chip short of workgroups
+  int64_t per = most;
+  while (per > 4 && (int64_t)images * t.slabs * ((q.HW + t.ty * per - 1) / (t.ty * per)) < 4 * ctx->cus) per >>= 1;
   t.pix = (int)(t.ty * per);
   t.chunks = (q.HW + t.pix - 1) / t.pix;
   return t;
 }
 struct SplitPlan {
-  LastTile t;
-  int chunks, pix, images;   // images of one batch
-  unsigned blocks;           // workgroups per image of the layout's kernels, in quarters of a workgroup channels first
+  LastTile sum, out;         // channels last: tiles of the sums and of the result
+  int chunks, pix, images;   // of the sums; images of one batch
+  unsigned sum_blocks, out_blocks;   // workgroups per image (channels first: quarters of one)
 };
-static SplitPlan split_plan(const DeviceCtx* ctx, const NormGeom& q, int tensors) {
+static SplitPlan split_plan(const DeviceCtx* ctx, const NormGeom& q) {
   SplitPlan s;
-  s.t = last_tile(ctx, q);
-  s.pix = q.last ? s.t.pix : kPlane;
+  const int n = q.N;
+  s.sum = last_tile(ctx, q, (int)n, 32);
+  s.out = last_tile(ctx, q, (int)n, 8);
+  s.pix = q.last ? s.sum.pix : kPlane;
   s.chunks = (q.HW + s.pix - 1) / s.pix;
-  s.blocks = q.last ? (unsigned)s.t.slabs * s.chunks : (unsigned)q.C * s.chunks;
-  // the tensors of one batch stay in the 256 MB memory-side cache until the second read; no grid reaches 2^32 threads
-  const uint64_t image = (uint64_t)q.C * q.HW * 4 * tensors, cap = 160u << 20;
-  uint64_t n = image >= cap ? 1 : cap / image;
-  const uint64_t most = (1u << 23) / (s.blocks > (unsigned)q.G ? s.blocks : (unsigned)q.G);
-  if (n > most) n = most > 0 ? most : 1;
-  s.images = n < (uint64_t)q.N ? (int)n : q.N;
+  s.sum_blocks = q.last ? (unsigned)s.sum.slabs * s.chunks : (unsigned)q.C * s.chunks;
+  s.out_blocks = q.last ? (unsigned)s.out.slabs * s.out.chunks : (unsigned)q.C * s.chunks;
+  const uint64_t most = (1u << 23) / std::max({s.sum_blocks, s.out_blocks, (unsigned)q.G});   // no grid reaches 2^32 threads
+  s.images = (int)std::max<uint64_t>(1, std::min<uint64_t>(n, most));
   return s;
 }
 
@@ -1055,37 +1312,45 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   if (st != LNN_OK) return st;
   const uint64_t n = (uint64_t)q.N * q.C * q.HW;
   // blocks of 32 lie inside a plane (channels first), a pixel's channels (last) or a row (one pixel): written on the way
-  const bool whole = (!q.last ? q.HW : q.HW == 1 ? q.Cg : q.C) % 32 == 0;
+  const GatherPlan gp = gather_plan(q);
+  const bool whole = !gp.T && (!q.last ? q.HW : q.HW == 1 ? q.Cg : q.C) % 32 == 0;
   uint8_t* codes = x8 && whole ? static_cast<uint8_t*>(x8) : nullptr;
   uint8_t* bytes = codes ? codes + n : nullptr;
   ResPlan p;
   if (q.HW == 1 && row_plan(q).L) {
     LNN_ROW_CASES(row_plan(q), fwd_rows, ctx, q, x, gamma, beta, y, mean, rstd, codes, bytes)
-  } else if (res_plan(ctx, q, 16, &p)) {
+  } else if (gp.T) {
+    LNN_GATHER_CASES(gp, fwd_gather, ctx, q, gp.pt, x, gamma, beta, y, mean, rstd)
+  } else if (res_plan(q, q.HW % 4 == 0 ? 16 : 13, 16, &p)) {
     for (; q.row0 < (uint32_t)(q.N * q.G); q.row0 += kMaxRows) {
       LNN_RES_CASES(p, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
-        case 256 * 32 + 16: fwd_res<256, 16>(ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes); break;
-        default: fwd_res<1024, 16>(ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes);
+        LNN_RES_CASE(512, 16, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
+        LNN_RES_CASE(1024, 10, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
+        LNN_RES_CASE(1024, 13, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
+        LNN_RES_CASE(1024, 16, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
+        default: return set_error(LNN_ERR_INVALID, "group_norm: no kernel for this plan");
       }
     }
   } else {
-    const SplitPlan s = split_plan(ctx, q, 2);
+    const SplitPlan s = split_plan(ctx, q);
+    const bool four = (q.last ? q.C : q.HW) % 4 == 0;   // no tensor of fewer than four elements comes here
     st = ensure_workspace(ctx, (uint64_t)s.images * s.chunks * q.C * 8);
     if (st != LNN_OK) return st;
     float2* part = static_cast<float2*>(ctx->ws);
     for (; q.n0 < q.N; q.n0 += s.images) {
       q.nb = q.N - q.n0 < s.images ? q.N - q.n0 : s.images;
-      const unsigned blocks = q.last ? q.nb * s.blocks : (q.nb * s.blocks + 3) / 4;
+      const unsigned blocks = q.last ? q.nb * s.sum_blocks : (q.nb * s.sum_blocks + 3) / 4;
+      const unsigned oblocks = q.last ? q.nb * s.out_blocks : (q.nb * s.out_blocks + 3) / 4;
       if (q.last)
-        hipLaunchKernelGGL(gn_stats_last_kernel, dim3(blocks), dim3(256), 0, ctx->stream, q, s.t, x, part);
+        hipLaunchKernelGGL(four ? gn_stats_last_kernel<G4> : gn_stats_last_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, part);
       else
-        hipLaunchKernelGGL(gn_stats_first_kernel, dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, part);
+        hipLaunchKernelGGL(four ? gn_stats_first_kernel<G4> : gn_stats_first_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, part);
       hipLaunchKernelGGL(gn_finish_kernel, dim3((unsigned)(q.nb * q.G)), dim3(256), 0, ctx->stream, q, s.chunks, s.pix, part, mean, rstd);
       if (q.last)
-        hipLaunchKernelGGL(codes ? gn_apply_last_kernel<true> : gn_apply_last_kernel<false>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.t, x,
+        hipLaunchKernelGGL((codes ? gn_apply_last_kernel<G4, true> : four ? gn_apply_last_kernel<G4, false> : gn_apply_last_kernel<GANY, false>), dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x,
                            gamma, beta, mean, rstd, y, codes, bytes);
       else
-        hipLaunchKernelGGL(codes ? gn_apply_first_kernel<true> : gn_apply_first_kernel<false>, dim3(blocks), dim3(256), 0, ctx->stream, q,
+        hipLaunchKernelGGL((codes ? gn_apply_first_kernel<G4, true> : four ? gn_apply_first_kernel<G4, false> : gn_apply_first_kernel<GANY, false>), dim3(oblocks), dim3(256), 0, ctx->stream, q,
                            s.chunks, x, gamma, beta, mean, rstd, y, codes, bytes);
     }
   }
@@ -1095,21 +1360,24 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
 
 template <class SRC>
 static void bwd_split(DeviceCtx* ctx, NormGeom q, const SplitPlan& s, SRC x, const float* gamma, const float* beta, const float* mean,
-                      const float* rstd, const float* dy, float* dx, int beta_dx, float* pa, float* pb, float2* s12) {
+                      const float* rstd, const float* dy, float* dx, int beta_dx, float* pa, float* pb, float2* s12, int K, float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta) {
+  const bool four = (q.last ? q.C : q.HW) % 4 == 0;   // no tensor of fewer than four elements comes here
   for (; q.n0 < q.N; q.n0 += s.images) {
     q.nb = q.N - q.n0 < s.images ? q.N - q.n0 : s.images;
-    const unsigned blocks = q.last ? q.nb * s.blocks : (q.nb * s.blocks + 3) / 4;
+    const unsigned blocks = q.last ? q.nb * s.sum_blocks : (q.nb * s.sum_blocks + 3) / 4;
+    const unsigned oblocks = q.last ? q.nb * s.out_blocks : (q.nb * s.out_blocks + 3) / 4;
     if (q.last)
-      hipLaunchKernelGGL((gn_sums_last_kernel<SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.t, x, gamma, beta, mean, rstd, dy, pa, pb);
+      hipLaunchKernelGGL((four ? gn_sums_last_kernel<G4, SRC> : gn_sums_last_kernel<GANY, SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, gamma, beta, mean, rstd, dy, pa, pb);
     else
-      hipLaunchKernelGGL((gn_sums_first_kernel<SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
+      hipLaunchKernelGGL((four ? gn_sums_first_kernel<G4, SRC> : gn_sums_first_kernel<GANY, SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
     if (!dx) continue;
-    hipLaunchKernelGGL(gn_finish_dx_kernel, dim3((unsigned)(q.nb * q.G)), dim3(256), 0, ctx->stream, q, s.chunks, gamma, pa, pb, s12);
+    hipLaunchKernelGGL(gn_finish_dx_kernel, dim3((unsigned)(q.nb * q.G + (K ? (q.C + 31) / 32 : 0))), dim3(256), 0, ctx->stream, q, s.chunks, gamma,
+                       pa, pb, s12, K, dgamma, beta_dgamma, dbeta, beta_dbeta);
     if (q.last)
-      hipLaunchKernelGGL((gn_dx_last_kernel<SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.t, x, gamma, beta, mean, rstd, dy, s12, dx,
+      hipLaunchKernelGGL((four ? gn_dx_last_kernel<G4, SRC> : gn_dx_last_kernel<GANY, SRC>), dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x, gamma, beta, mean, rstd, dy, s12, dx,
                          beta_dx);
     else
-      hipLaunchKernelGGL((gn_dx_first_kernel<SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, s12,
+      hipLaunchKernelGGL((four ? gn_dx_first_kernel<G4, SRC> : gn_dx_first_kernel<GANY, SRC>), dim3(oblocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, s12,
                          dx, beta_dx);
   }
 }
@@ -1125,7 +1393,8 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   const uint8_t* codes = static_cast<const uint8_t*>(x8);
   const uint8_t* bytes = x8 ? codes + blocks8((uint64_t)q.N * q.C * q.HW) * 32 : nullptr;
   // K rows of channel sums, and room for the rows that many of them are first brought down to
-  enum { kRows, kRes, kSplit } path;
+  enum { kRows, kRes, kGather, kSplit } path;
+  const GatherPlan gp = gather_plan(q);
   ResPlan p;
   SplitPlan s;
   uint64_t K;
@@ -1133,12 +1402,15 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
     path = kRows;
     const int slots = 256 / row_plan(q).L;   // four rows or more per slot, about eight workgroups per compute unit
     K = std::min<uint64_t>(((uint64_t)q.N + 4 * slots - 1) / (4 * slots), ((uint64_t)8 * ctx->cus + q.G - 1) / q.G);
-  } else if (res_plan(ctx, q, 8, &p)) {
+  } else if (res_plan(q, 8, q.HW % 4 != 0 ? 8 : x8 ? 13 : 10, &p)) {
     path = kRes;
+    K = q.N;
+  } else if (gp.T) {
+    path = kGather;
     K = q.N;
   } else {
     path = kSplit;
-    s = split_plan(ctx, q, 3);
+    s = split_plan(ctx, q);
     K = (uint64_t)q.N * s.chunks;
   }
   const uint64_t per = std::max<uint64_t>(256, (K + 511) / 512), K2 = K > 512 ? (K + per - 1) / per : 0;
@@ -1150,19 +1422,25 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   float* qa = pb + sums;
   float* qb = qa + K2 * q.C;
   float2* s12 = reinterpret_cast<float2*>(qb + K2 * q.C);   // an even number of floats behind the start
+  // dgamma and dbeta in the launch that finishes the rows' sums, where there is one such launch
+  const bool with = params && path == kSplit && dx && K2 == 0 && s.images == q.N;
   if (path == kRows) {
     LNN_ROW_CASES(row_plan(q), bwd_rows, ctx, q, (int)K, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa)
   } else if (path == kRes) {
     for (; q.row0 < (uint32_t)(q.N * q.G); q.row0 += kMaxRows) {
       LNN_RES_CASES(p, bwd_res, ctx, q, p.un, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa)
+        default: return set_error(LNN_ERR_INVALID, "group_norm: no kernel for this plan");
       }
     }
+  } else if (path == kGather) {
+    LNN_GATHER_CASES(gp, bwd_gather, ctx, q, gp.pt, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa)
   } else if (x8) {
-    bwd_split(ctx, q, s, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12);
+    bwd_split(ctx, q, s, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, with ? (int)K : 0, dgamma, beta_dgamma, dbeta,
+              beta_dbeta);
   } else {
-    bwd_split(ctx, q, s, SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12);
+    bwd_split(ctx, q, s, SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, with ? (int)K : 0, dgamma, beta_dgamma, dbeta, beta_dbeta);
   }
-  if (params) {
+  if (params && !with) {
     const unsigned cols = (unsigned)((q.C + 31) / 32);
     if (K2) {
       hipLaunchKernelGGL(gn_params_kernel, dim3(cols, (unsigned)K2), dim3(256), 0, ctx->stream, (int)K, (int)per, q.C, pa, pb, qa, 0, qb, 0);

@@ -168,3 +168,16 @@ def test_wgrad_nonfinite_stays_in_its_place(hip):
     want[32:64, :] = True
     want[:, 7] = True
     assert np.array_equal(bad, want)
+
+
+@pytest.mark.parametrize('shape', [(20000, 2, 3, 2), (1, 600000, 2, 3)])
+def test_wgrad_in_parts(hip, shape):
+    """More batch items, and more rows, than one launch lays out: whole numbers, exact, written and accumulated."""
+    say(f'wgrad8 in parts {shape}')
+    batch, rows, K, M = shape
+    rs = np.random.RandomState(16)
+    x = rs.randint(-3, 4, (batch, rows, K)).astype(np.float32)
+    dy = rs.randint(-4, 5, (batch, rows, M)).astype(np.float32)
+    ref = np.matmul(x.transpose(0, 2, 1).astype(np.float64), dy.astype(np.float64))     # below 600000 * 12 < 2^24
+    assert np.array_equal(wgrad(hip, x, dy), ref)
+    assert np.array_equal(wgrad(hip, x, dy, prefill=3.0), ref + 3)
