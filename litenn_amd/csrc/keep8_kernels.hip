@@ -75,9 +75,9 @@ int launch_decode8(DeviceCtx* ctx, uint64_t n, const void* src, float* dst) {
 // pipe, every product exact and every sum fp32: what an fp32 product of the same values would give, at three times the
 // bf16 work, which is a fifth of the fp32 pipe's time.
 //
-// Measured: 8192 rows, 4096 x 4096: 0.72 ms = 1.15 PFLOP/s of bf16 work, 380 TFLOP/s of the product (the fp32 pipe's product of
-// decoded values: 2.0 ms), the main kernel alone 0.63 ms, 1.3 PFLOP/s: as the library's bf16 product of that size runs here.
-// Bound: the matrix pipe; the first pass, 435 MB of traffic, is the rest.
+// Measured: 8192 rows, 4096 x 4096: 0.69 ms = 1.2 PFLOP/s of bf16 work, 400 TFLOP/s of the product (the fp32 pipe's product of
+// decoded values: 2.0 ms), the main kernel alone 0.61 ms, 1.35 PFLOP/s: as a library's bf16 product of that size runs here.
+// Bound: the matrix pipe; the first pass, 435 MB of traffic in 77 us, is the rest.
 //
 // First pass: both operands are laid out as the matrix instruction reads them, 1 KB per fragment of 32 columns x 16 rows
 // (lane l holds column l % 32, rows 8 (l / 32) .. + 7), rows and columns padded with zeros to whole tiles.  The main kernel
@@ -92,49 +92,64 @@ struct W8 {
   int b0, r0, all;         // its first batch item and row; rows of the whole operand
   int steps;               // of 32 rows
   int ipan, jpan;    // panels of 32 columns of X and dO, whole tiles
-  uint32_t xblocks, xsize, osize;   // blocks of the 8-bit copy; elements of X and dO
+  uint32_t xblocks, xsize;   // blocks of the 8-bit copy; elements of X
 };
 
 __device__ __forceinline__ uint32_t hi16(uint32_t lo, uint32_t hi) { return (lo >> 16) | (hi & 0xffff0000u); }   // two bf16 of two fp32
 
-// A workgroup lays out 16 rows x 512 columns of X (its first xwgs pieces of 16 rows) or dO at a time; a thread 8 rows x 4
-// columns.
-template <int MX, int MO>
-__device__ __forceinline__ void w8_pack(const W8& w, int b, int r16, bool isx, int pan, const uint8_t* x8, const float* dO, uint4* ap,
-                                        uint4* bp) {
-  const int half = (threadIdx.x >> 3) & 1, quad = threadIdx.x & 7;
-  const int pans = isx ? w.ipan : w.jpan, cols = isx ? w.K : w.M;
-  const int c = pan * 32 + quad * 4, cnt = min(max(cols - c, 0), 4), r0 = r16 * 16 + half * 8;
+// A workgroup lays out 16 rows x 512 columns of X (the first xwgs pieces of 16 rows) or dO at a time.
+//
+// X: a thread takes 8 rows x 4 columns, words of four codes.
+template <int MX>
+__device__ __forceinline__ void w8_pack_x(const W8& w, int b, int r16, int pan0, const uint8_t* x8, uint4* ap) {
+  const int pan = pan0 + threadIdx.x / 16, half = (threadIdx.x >> 3) & 1, quad = threadIdx.x & 7;
+  if (pan >= w.ipan) return;
+  const int c = pan * 32 + quad * 4, cnt = min(max(w.K - c, 0), 4), r0 = r16 * 16 + half * 8;
+  const Src8 x = {x8, x8 + (uint64_t)w.xblocks * 32};
   float v[8][4];
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int n = r0 + r < w.rows ? cnt : 0;
-    const uint32_t at = ((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * cols + c;
-    if (isx)
-      Src8{x8, x8 + (uint64_t)w.xblocks * 32}.load<MX>(at, n, w.xsize, v[r]);
-    else
-      load4<MO>(dO, at, n, w.osize, v[r]);
-  }
-  const uint64_t frag = ((uint64_t)b * 2 * w.steps + r16) * pans + pan;
-  const int lane = half * 32 + quad * 4;
+  for (int r = 0; r < 8; ++r)
+    x.load<MX>(((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * w.K + c, r0 + r < w.rows ? cnt : 0, w.xsize, v[r]);
+  uint4* o = ap + (((uint64_t)b * 2 * w.steps + r16) * w.ipan + pan) * 64 + half * 32 + quad * 4;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
+    uint32_t h[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) h[r] = __float_as_uint(v[r][k]);
+    o[k] = make_uint4(hi16(h[0], h[1]), hi16(h[2], h[3]), hi16(h[4], h[5]), hi16(h[6], h[7]));
+  }
+}
+// dO: a thread takes 8 rows of one column, so that a wavefront stores each part of a fragment as one kilobyte (with 4 columns to a
+// thread, stores of 16 bytes every 64: 146 us for this pass
+// at 8192 x 4096 x 4096, 77 so)
+__device__ __forceinline__ void w8_pack_o(const W8& w, int b, int r16, int pan0, const float* dO, uint4* bp) {
+  const int half = (threadIdx.x >> 5) & 1, r0 = r16 * 16 + half * 8;
+  float v[4][8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = (pan0 + j * 4 + (int)(threadIdx.x >> 6)) * 32 + (threadIdx.x & 31);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const bool in = c < w.M && r0 + r < w.rows;
+      const float d = dO[in ? ((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * w.M + c : 0u];
+      v[j][r] = in ? d : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int pan = pan0 + j * 4 + (int)(threadIdx.x >> 6);
     uint32_t h[8], m[8], l[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      h[r] = __float_as_uint(v[r][k]);
-      if (!isx) {
-        const bool odd = (h[r] & 0x7f800000u) == 0x7f800000u;   // infinity and NaN have no rest
-        const float rest = odd ? 0.0f : v[r][k] - __uint_as_float(h[r] & 0xffff0000u);
-        if (odd && (h[r] & 0x7fffffu)) h[r] = 0x7fc00000u;
-        m[r] = __float_as_uint(rest);
-        l[r] = __float_as_uint(rest - __uint_as_float(m[r] & 0xffff0000u));
-      }
+      h[r] = __float_as_uint(v[j][r]);
+      const bool odd = (h[r] & 0x7f800000u) == 0x7f800000u;   // infinity and NaN have no rest
+      const float rest = odd ? 0.0f : v[j][r] - __uint_as_float(h[r] & 0xffff0000u);
+      if (odd && (h[r] & 0x7fffffu)) h[r] = 0x7fc00000u;
+      m[r] = __float_as_uint(rest);
+      l[r] = __float_as_uint(rest - __uint_as_float(m[r] & 0xffff0000u));
     }
-    if (isx) {
-      ap[frag * 64 + lane + k] = make_uint4(hi16(h[0], h[1]), hi16(h[2], h[3]), hi16(h[4], h[5]), hi16(h[6], h[7]));
-    } else {
-      uint4* o = bp + frag * 192 + lane + k;
+    if (pan < w.jpan) {
+      uint4* o = bp + (((uint64_t)b * 2 * w.steps + r16) * w.jpan + pan) * 192 + (threadIdx.x & 63);
       o[0] = make_uint4(hi16(h[0], h[1]), hi16(h[2], h[3]), hi16(h[4], h[5]), hi16(h[6], h[7]));
       o[64] = make_uint4(hi16(m[0], m[1]), hi16(m[2], m[3]), hi16(m[4], m[5]), hi16(m[6], m[7]));
       o[128] = make_uint4(hi16(l[0], l[1]), hi16(l[2], l[3]), hi16(l[4], l[5]), hi16(l[6], l[7]));
@@ -142,14 +157,15 @@ __device__ __forceinline__ void w8_pack(const W8& w, int b, int r16, bool isx, i
   }
 }
 
-template <int MX, int MO>
+template <int MX>
 __global__ __launch_bounds__(256) void w8_pack_kernel(W8 w, int xwgs, int owgs, const uint8_t* x8, const float* dO, uint4* ap, uint4* bp) {
   const uint32_t wgs = xwgs + owgs, pieces = (uint32_t)w.batch * 2 * w.steps * wgs;
   for (uint32_t u = blockIdx.x; u < pieces; u += gridDim.x) {
     const uint32_t k = u / wgs, y = u - k * wgs;
-    const bool isx = y < (uint32_t)xwgs;
-    const int pan = (isx ? y : y - xwgs) * 16 + threadIdx.x / 16;
-    if (pan < (isx ? w.ipan : w.jpan)) w8_pack<MX, MO>(w, k / (2 * w.steps), k % (2 * w.steps), isx, pan, x8, dO, ap, bp);
+    if (y < (uint32_t)xwgs)
+      w8_pack_x<MX>(w, k / (2 * w.steps), k % (2 * w.steps), y * 16, x8, ap);
+    else
+      w8_pack_o(w, k / (2 * w.steps), k % (2 * w.steps), (y - xwgs) * 16, dO, bp);
   }
 }
 
@@ -285,14 +301,10 @@ static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* 
   const int xwgs = (w.ipan + 15) / 16, owgs = (w.jpan + 15) / 16;
   const uint64_t pieces = (uint64_t)batch * 2 * w.steps * (xwgs + owgs);
   const dim3 pgrid((unsigned)std::min<uint64_t>(pieces, 1u << 20));
-  // rows of whole groups of four are read without shifts; dO of fewer than four elements one by one
-  const bool x4 = K % 4 == 0, o4 = M % 4 == 0;
-  if (w.osize < 4)
-    hipLaunchKernelGGL((w8_pack_kernel<GANY, GTINY>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
-  else if (x4 && o4)
-    hipLaunchKernelGGL((w8_pack_kernel<G4, G4>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
+  if (K % 4 == 0)   // rows of X are whole groups of four: no shifts
+    hipLaunchKernelGGL((w8_pack_kernel<G4>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
   else
-    hipLaunchKernelGGL((w8_pack_kernel<GANY, GANY>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
+    hipLaunchKernelGGL((w8_pack_kernel<GANY>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
   const int64_t total = (int64_t)ti * tj * splits * batch;
   const dim3 grid((unsigned)((total + 7) / 8 * 8));
   float* out = splits > 1 ? pp : dW;
@@ -313,7 +325,6 @@ int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void*
   w.M = M;
   w.all = rows;
   w.xsize = (uint32_t)batch * rows * K;
-  w.osize = (uint32_t)batch * rows * M;
   w.xblocks = (uint32_t)blocks8(w.xsize);
   // The laid-out operands of one launch stay below a gigabyte: many small products go in groups, one product of very
   // many rows in runs of rows, each added to the one before.
