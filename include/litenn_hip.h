@@ -324,7 +324,7 @@ int lnn_random_normal_f32(int dev, float* out, uint64_t n, uint32_t seed, double
  *        xh = (x - mean[row]) * rstd[row];   y = act(gamma[c] * xh + beta[c])
  *        rstd = 1 / sqrt(var + eps), var the mean squared distance from the mean
  *      act: LNN_ACT_NONE, LNN_ACT_LEAKY_RELU with any slope (0: ReLU; the derivative at 0 is 1, as lnn_ew_bwd_f32's),
- *      LNN_ACT_SILU.  gamma / beta: C values, or NULL for ones / zeros.  eps > 0. */
+ *      LNN_ACT_SILU.  gamma / beta: C values, or NULL for ones / zeros.  eps > 0.  At most 4194304 channels. */
 typedef struct lnn_group_norm_desc {
   int32_t N, C, HW, groups;
   int32_t channels_last, act;
@@ -344,8 +344,7 @@ int lnn_group_norm_bwd_f32(int dev, const lnn_group_norm_desc* d, const float* x
 
 /* ---- activations kept in 8 bits between the forward and the backward pass.
  *      Every 32 elements that follow each other in memory share a power of two 2^e: with a the largest magnitude among
- *      them, e is the smallest whole number for which a * 2^-e < 127.5, kept within [-126, 121] (e of a power-of-two range:
- *      64 <= a * 2^-e < 127.5 wherever neither limit acts).  Codes are round-half-even(x * 2^-e) as int8, within +-127; an
+ *      them, e is the smallest whole number for which a * 2^-e < 127.5, kept within [-126, 121].  Codes are round-half-even(x * 2^-e) as int8, within +-127; an
  *      element reads back as code * 2^e, off by at most half of 2^e.  A copy of n elements is ceil(n / 32) * 32 codes (the
  *      last block padded with zeros) followed by ceil(n / 32) exponent bytes: e + 127, or 0 for a block of zeros, or 255
  *      for a block that holds an infinity or a NaN, all of which reads back as NaN. */

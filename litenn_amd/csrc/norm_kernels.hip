@@ -19,8 +19,8 @@ struct NormGeom {
   int n0, nb;           // images of this launch
   float slope, eps;
   float d, inv_d;       // D and 1 / D; means are divided by D: a row of equal values then has exactly their mean
-  uint32_t D, size;   // elements of a row and of the tensor
-  uint32_t row0;      // row0: first row of this launch (a grid holds fewer than 2^32 threads)
+  uint32_t D, size;     // elements of a row and of the tensor
+  uint32_t row0;        // first row of this launch (a grid holds fewer than 2^32 threads)
 };
 
 // 1 / (1 + exp(-p)) by the one-instruction power of two and reciprocal (one unit in the last place each).  Rounding
@@ -59,7 +59,9 @@ __device__ __forceinline__ void slope4(int silu, float slope, const float* p, fl
 // registers.  512 lanes: two rows or more to a compute unit, so that one is read while another is computed or written
 // (32 x 256 x 56 x 56 from 8 bits, forward + backward: 116 us against 130 with 1024 lanes and one row); 1024 where there are
 // fewer rows than compute units.  The loads of a row stand together, in front of everything that waits for them (67 -> 61 us).
-// Bound: memory.  32 x 128 x 56 x 56 forward 22 us, 4.7 TB/s; forward + backward with SiLU 61 us, 4.2 TB/s.  The row is dealt out in units of 2^ul lanes, each unit inside one channel plane (4 * 2^ul elements of it),
+// Bound: memory.  32 x 128 x 56 x 56 forward 22 us, 4.7 TB/s; forward + backward with SiLU 61 us, 4.2 TB/s.
+//
+// The row is dealt out in units of 2^ul lanes, each unit inside one channel plane (4 * 2^ul elements of it),
 // so gamma, beta and the channel sums of the backward pass belong to whole units and no element needs a division.
 struct Units {
   int ul, per, total;   // log2 lanes of a unit; units of a plane; units of the row
@@ -1121,7 +1123,7 @@ struct ResPlan {
   int T, V;
 };
 // most: groups per lane at 1024 lanes; most512: the same at 512
-static bool res_plan(const NormGeom& q, int most, int most512, ResPlan* p) {
+static bool res_plan(const DeviceCtx* ctx, const NormGeom& q, int most, int most512, ResPlan* p) {
   if (q.last) return false;
   // the shortest unit that holds a plane, or whole wavefronts
   p->un.ul = q.HW <= 4 ? 0 : q.HW <= 16 ? 2 : q.HW <= 64 ? 4 : 6;
@@ -1131,7 +1133,7 @@ static bool res_plan(const NormGeom& q, int most, int most512, ResPlan* p) {
   if (lanes > 1024u * most || p->un.total > 3500) return false;   // 3500: two sums per unit, gamma and beta in 64 KB of LDS
   p->un.dper = make_fastdiv((uint32_t)p->un.per);
   p->T = lanes <= 64 ? 64 : lanes <= 1024 ? 256 : lanes <= 512u * most512 ? 512 : 1024;
-  if (lanes > 1024 && q.N * q.G <= 256) p->T = 1024;   // fewer rows than compute units: more lanes to each
+  if (lanes > 1024 && q.N * q.G <= ctx->cus) p->T = 1024;   // fewer rows than compute units: more lanes to each
   static const int sizes[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 13, 16};
   for (int v : sizes)
     if (lanes <= (uint64_t)p->T * v) {
@@ -1151,7 +1153,11 @@ static void fwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const fl
     hipLaunchKernelGGL((gn_fwd_res_kernel<T, V, G4, true>), dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
                        mean, rstd, codes, bytes);
   else
-    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_fwd_res_kernel<T, V, G4, false> : q.size >= 4 ? gn_fwd_res_kernel<T, V, GANY, false> : gn_fwd_res_kernel<T, V, T == 64 ? GTINY : GANY, false>), dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
+    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_fwd_res_kernel<T, V, G4, false> :
+                            q.size >= 4 ? gn_fwd_res_kernel<T, V, GANY, false> :
+                            gn_fwd_res_kernel<T, V, T == 64 ? GTINY :
+                            GANY, false>),
+                           dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
                        mean, rstd, codes, bytes);
 }
 template <int T, int V>
@@ -1163,10 +1169,17 @@ static void bwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const fl
     hipLaunchKernelGGL((gn_bwd_res_kernel<T, V, G4, Src8, Hold8>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
                        Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
   else if (codes)
-    hipLaunchKernelGGL((q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, Src8, HoldF> : gn_bwd_res_kernel<T, V, T == 64 ? GTINY : GANY, Src8, HoldF>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
+    hipLaunchKernelGGL((q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, Src8, HoldF> :
+                            gn_bwd_res_kernel<T, V, T == 64 ? GTINY :
+                            GANY, Src8, HoldF>),
+                           dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
                        Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_bwd_res_kernel<T, V, G4, SrcF, HoldF> : q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, SrcF, HoldF> : gn_bwd_res_kernel<T, V, T == 64 ? GTINY : GANY, SrcF, HoldF>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un, SrcF{x}, gamma,
+    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_bwd_res_kernel<T, V, G4, SrcF, HoldF> :
+                            q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, SrcF, HoldF> :
+                            gn_bwd_res_kernel<T, V, T == 64 ? GTINY :
+                            GANY, SrcF, HoldF>),
+                           dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un, SrcF{x}, gamma,
                        beta, mean, rstd, dy, dx, beta_dx, part);
 }
 #define LNN_RES_CASE(T, V, F, ...) \
@@ -1219,7 +1232,11 @@ static void fwd_rows(DeviceCtx* ctx, const NormGeom& q, const float* x, const fl
   if (codes)
     hipLaunchKernelGGL((gn_fwd_rows_kernel<L, V, G4, true>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
   else
-    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_fwd_rows_kernel<L, V, G4, false> : q.C >= 4 ? gn_fwd_rows_kernel<L, V, GANY, false> : gn_fwd_rows_kernel<L, V, L == 4 ? GTINY : GANY, false>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
+    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_fwd_rows_kernel<L, V, G4, false> :
+                            q.C >= 4 ? gn_fwd_rows_kernel<L, V, GANY, false> :
+                            gn_fwd_rows_kernel<L, V, L == 4 ? GTINY :
+                            GANY, false>),
+                           dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
 }
 template <int L, int V>
 static void bwd_rows(DeviceCtx* ctx, const NormGeom& q, int chunks, const float* x, const uint8_t* codes, const uint8_t* bytes,
@@ -1227,10 +1244,18 @@ static void bwd_rows(DeviceCtx* ctx, const NormGeom& q, int chunks, const float*
                      float* part) {
   const unsigned blocks = (unsigned)chunks * q.G;
   if (codes)
-    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, Src8> : q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, Src8> : gn_bwd_rows_kernel<L, V, L == 4 ? GTINY : GANY, Src8>), dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, Src8{codes, bytes}, gamma, beta,
+    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, Src8> :
+                            q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, Src8> :
+                            gn_bwd_rows_kernel<L, V, L == 4 ? GTINY :
+                            GANY, Src8>),
+                           dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, Src8{codes, bytes}, gamma, beta,
                        mean, rstd, dy, dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, SrcF> : q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, SrcF> : gn_bwd_rows_kernel<L, V, L == 4 ? GTINY : GANY, SrcF>), dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, SrcF{x}, gamma, beta, mean, rstd,
+    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, SrcF> :
+                            q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, SrcF> :
+                            gn_bwd_rows_kernel<L, V, L == 4 ? GTINY :
+                            GANY, SrcF>),
+                           dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, SrcF{x}, gamma, beta, mean, rstd,
                        dy, dx, beta_dx, part);
 }
 
@@ -1273,7 +1298,7 @@ static void bwd_gather(DeviceCtx* ctx, const NormGeom& q, int pt, const float* x
 }
 
 // The tile of the channels-last kernels, and the chunks of either layout.
-static LastTile last_tile(const DeviceCtx* ctx, const NormGeom& q, int images, int most) {
+static LastTile last_tile(const DeviceCtx* ctx, const NormGeom& q, int most) {
   LastTile t;
   const int cv = (q.C + 3) / 4;
   t.tx = cv < 256 ? cv : 256;
@@ -1281,7 +1306,7 @@ static LastTile last_tile(const DeviceCtx* ctx, const NormGeom& q, int images, i
   t.ty = 256 / t.tx;
   // a lane walks over `most` pixels, fewer where that leaves the chip short of workgroups
   int64_t per = most;
-  while (per > 4 && (int64_t)images * t.slabs * ((q.HW + t.ty * per - 1) / (t.ty * per)) < 4 * ctx->cus) per >>= 1;
+  while (per > 4 && (int64_t)q.N * t.slabs * ((q.HW + t.ty * per - 1) / (t.ty * per)) < 4 * ctx->cus) per >>= 1;
   t.pix = (int)(t.ty * per);
   t.chunks = (q.HW + t.pix - 1) / t.pix;
   return t;
@@ -1293,15 +1318,14 @@ struct SplitPlan {
 };
 static SplitPlan split_plan(const DeviceCtx* ctx, const NormGeom& q) {
   SplitPlan s;
-  const int n = q.N;
-  s.sum = last_tile(ctx, q, (int)n, 32);
-  s.out = last_tile(ctx, q, (int)n, 8);
+  s.sum = last_tile(ctx, q, 32);
+  s.out = last_tile(ctx, q, 8);
   s.pix = q.last ? s.sum.pix : kPlane;
   s.chunks = (q.HW + s.pix - 1) / s.pix;
   s.sum_blocks = q.last ? (unsigned)s.sum.slabs * s.chunks : (unsigned)q.C * s.chunks;
   s.out_blocks = q.last ? (unsigned)s.out.slabs * s.out.chunks : (unsigned)q.C * s.chunks;
   const uint64_t most = (1u << 23) / std::max({s.sum_blocks, s.out_blocks, (unsigned)q.G});   // no grid reaches 2^32 threads
-  s.images = (int)std::max<uint64_t>(1, std::min<uint64_t>(n, most));
+  s.images = (int)std::max<uint64_t>(1, std::min<uint64_t>(q.N, most));
   return s;
 }
 
@@ -1321,7 +1345,7 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
     LNN_ROW_CASES(row_plan(q), fwd_rows, ctx, q, x, gamma, beta, y, mean, rstd, codes, bytes)
   } else if (gp.T) {
     LNN_GATHER_CASES(gp, fwd_gather, ctx, q, gp.pt, x, gamma, beta, y, mean, rstd)
-  } else if (res_plan(q, q.HW % 4 == 0 ? 16 : 13, 16, &p)) {
+  } else if (res_plan(ctx, q, q.HW % 4 == 0 ? 16 : 13, 16, &p)) {
     for (; q.row0 < (uint32_t)(q.N * q.G); q.row0 += kMaxRows) {
       LNN_RES_CASES(p, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
         LNN_RES_CASE(512, 16, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
@@ -1347,10 +1371,16 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
         hipLaunchKernelGGL(four ? gn_stats_first_kernel<G4> : gn_stats_first_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, part);
       hipLaunchKernelGGL(gn_finish_kernel, dim3((unsigned)(q.nb * q.G)), dim3(256), 0, ctx->stream, q, s.chunks, s.pix, part, mean, rstd);
       if (q.last)
-        hipLaunchKernelGGL((codes ? gn_apply_last_kernel<G4, true> : four ? gn_apply_last_kernel<G4, false> : gn_apply_last_kernel<GANY, false>), dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x,
+        hipLaunchKernelGGL((codes ? gn_apply_last_kernel<G4, true> :
+                                four ? gn_apply_last_kernel<G4, false> :
+                                gn_apply_last_kernel<GANY, false>),
+                               dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x,
                            gamma, beta, mean, rstd, y, codes, bytes);
       else
-        hipLaunchKernelGGL((codes ? gn_apply_first_kernel<G4, true> : four ? gn_apply_first_kernel<G4, false> : gn_apply_first_kernel<GANY, false>), dim3(oblocks), dim3(256), 0, ctx->stream, q,
+        hipLaunchKernelGGL((codes ? gn_apply_first_kernel<G4, true> :
+                                four ? gn_apply_first_kernel<G4, false> :
+                                gn_apply_first_kernel<GANY, false>),
+                               dim3(oblocks), dim3(256), 0, ctx->stream, q,
                            s.chunks, x, gamma, beta, mean, rstd, y, codes, bytes);
     }
   }
@@ -1367,17 +1397,25 @@ static void bwd_split(DeviceCtx* ctx, NormGeom q, const SplitPlan& s, SRC x, con
     const unsigned blocks = q.last ? q.nb * s.sum_blocks : (q.nb * s.sum_blocks + 3) / 4;
     const unsigned oblocks = q.last ? q.nb * s.out_blocks : (q.nb * s.out_blocks + 3) / 4;
     if (q.last)
-      hipLaunchKernelGGL((four ? gn_sums_last_kernel<G4, SRC> : gn_sums_last_kernel<GANY, SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, gamma, beta, mean, rstd, dy, pa, pb);
+      hipLaunchKernelGGL((four ? gn_sums_last_kernel<G4, SRC> :
+                              gn_sums_last_kernel<GANY, SRC>),
+                             dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, gamma, beta, mean, rstd, dy, pa, pb);
     else
-      hipLaunchKernelGGL((four ? gn_sums_first_kernel<G4, SRC> : gn_sums_first_kernel<GANY, SRC>), dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
+      hipLaunchKernelGGL((four ? gn_sums_first_kernel<G4, SRC> :
+                              gn_sums_first_kernel<GANY, SRC>),
+                             dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
     if (!dx) continue;
     hipLaunchKernelGGL(gn_finish_dx_kernel, dim3((unsigned)(q.nb * q.G + (K ? (q.C + 31) / 32 : 0))), dim3(256), 0, ctx->stream, q, s.chunks, gamma,
                        pa, pb, s12, K, dgamma, beta_dgamma, dbeta, beta_dbeta);
     if (q.last)
-      hipLaunchKernelGGL((four ? gn_dx_last_kernel<G4, SRC> : gn_dx_last_kernel<GANY, SRC>), dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x, gamma, beta, mean, rstd, dy, s12, dx,
+      hipLaunchKernelGGL((four ? gn_dx_last_kernel<G4, SRC> :
+                              gn_dx_last_kernel<GANY, SRC>),
+                             dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x, gamma, beta, mean, rstd, dy, s12, dx,
                          beta_dx);
     else
-      hipLaunchKernelGGL((four ? gn_dx_first_kernel<G4, SRC> : gn_dx_first_kernel<GANY, SRC>), dim3(oblocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, s12,
+      hipLaunchKernelGGL((four ? gn_dx_first_kernel<G4, SRC> :
+                              gn_dx_first_kernel<GANY, SRC>),
+                             dim3(oblocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, s12,
                          dx, beta_dx);
   }
 }
@@ -1402,7 +1440,7 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
     path = kRows;
     const int slots = 256 / row_plan(q).L;   // four rows or more per slot, about eight workgroups per compute unit
     K = std::min<uint64_t>(((uint64_t)q.N + 4 * slots - 1) / (4 * slots), ((uint64_t)8 * ctx->cus + q.G - 1) / q.G);
-  } else if (res_plan(q, 8, q.HW % 4 != 0 ? 8 : x8 ? 13 : 10, &p)) {
+  } else if (res_plan(ctx, q, 8, q.HW % 4 != 0 ? 8 : x8 ? 13 : 10, &p)) {
     path = kRes;
     K = q.N;
   } else if (gp.T) {

@@ -111,7 +111,9 @@ SHAPES = [  # N, C, HW, groups
     (1, 1, 3, 1), (1, 8, 1, 1), (1, 64, 196, 8), (2, 6, 35, 3), (3, 60, 37 * 41, 12), (2, 32, 64, 32), (1, 4, 63, 2), (5, 12, 9, 4),
     (2, 128, 56 * 56, 32), (1, 3, 1000, 1), (4, 96, 49, 8), (2, 320, 256, 32), (1, 16, 70 * 71, 1), (2, 40, 33, 5), (7, 24, 1, 3),
     (300, 96, 1, 4), (33, 512, 1, 32), (64, 1000, 1, 1), (9, 34, 2, 17), (2, 1028, 5, 4), (1, 2, 65536, 2), (1, 64, 16384, 2),
-    (600, 8, 4, 2), (5, 2048, 1, 1), (3, 5000, 1, 1), (2, 20000, 1, 2), (3, 6, 90000, 3), (2, 8000, 3, 1), (1, 33, 70000, 1), (1, 2080, 40, 5)]
+    (600, 8, 4, 2), (5, 2048, 1, 1), (3, 5000, 1, 1), (2, 20000, 1, 2), (3, 6, 90000, 3), (2, 8000, 3, 1), (1, 33, 70000, 1), (1, 2080, 40, 5),
+    (1, 1, 1, 1), (1, 1, 2, 1), (1, 3, 1, 1), (50, 3, 1, 1), (50, 3, 1, 3), (9, 2, 1, 1), (40, 5, 1, 5), (2, 3, 9001, 1), (150, 8, 3001, 2),
+    (260, 26, 1000, 1), (270, 26, 999, 1), (3, 7, 1, 1), (70, 1, 19, 1)]
 
 
 @pytest.mark.parametrize('shape', SHAPES)
