@@ -16,8 +16,9 @@ def keep8(t):
 
     The gradient functions of group_norm and of a matmul's second operand (a dense layer's weight) read the copy as it
     is; every other reader of t, forward or backward, gets the rounded values decoded into fp32, which backward() lets go
-    again as soon as the tensor's gradient functions have run.  Writing to t (set, fill, output_t=) ends the 8-bit
-    state.  Returns t."""
+    again as soon as the tensor's gradient functions have run.  A value below half a step reads back as 0, also for a
+    (leaky) ReLU whose gradient takes the sign from t.  Writing to t (set, fill, output_t=) ends the 8-bit state.
+    Returns t."""
     check_keep8(t)
     for buf in t._get_buffers():
         buf.keep8()
