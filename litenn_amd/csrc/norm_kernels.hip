@@ -574,7 +574,7 @@ __global__ __launch_bounds__(T) void gn_bwd_gather_kernel(NormGeom q, int pt, SR
 // second time from its end backwards, where what the first reading left in the 256 MB memory-side cache still is.
 // Taking the images in batches that fit that cache was slower (16 x 128 x 128 x 256 forward: 276 us in batches of 96 MB, 208 of
 // 160 MB, 166 in one): the cache saves less than each batch's three short launches cost.
-// 16 x 128 x 128 x 256 forward 160 us = 805 MB at 5.0 TB/s; 8 x 64 x 64 x 320 step from 8 bits 87 us.
+// 16 x 128 x 128 x 256 forward 160 us = 805 MB at 5.0 TB/s; 8 x 64 x 64 x 320 step from 8 bits 85 us.
 //
 // Means and sums of squared distances of two sets join as
 //   n = na + nb, d = mb - ma:  m = ma + d nb / n,  M = Ma + Mb + d^2 na nb / n
@@ -841,12 +841,14 @@ __global__ __launch_bounds__(256) void gn_stats_last_kernel(NormGeom q, LastTile
 }
 
 // Statistics of row (n, g) from those of its channels and chunks of `pix` pixels.
-__global__ __launch_bounds__(256) void gn_finish_kernel(NormGeom q, int chunks, int pix, const float2* part, float* mean, float* rstd) {
-  __shared__ Stat sh[4];
+// T lanes: 1024 where a row has more channel-chunks than one walk of 256 (2 x 22263 x 54 in one group, step: 99 -> 57 us)
+template <int T>
+__global__ __launch_bounds__(T) void gn_finish_kernel(NormGeom q, int chunks, int pix, const float2* part, float* mean, float* rstd) {
+  __shared__ Stat sh[T / 64];
   const uint32_t n = blockIdx.x / q.G, g = blockIdx.x % q.G;   // n: image of the batch
   Stat s = {0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int j = threadIdx.x; j < chunks * q.Cg; j += 256) {
+  for (int j = threadIdx.x; j < chunks * q.Cg; j += T) {
     const int chunk = j / q.Cg, c = j - chunk * q.Cg;
     const float2 e = part[(n * chunks + chunk) * q.C + g * q.Cg + c];
     s = join(s, Stat{(float)min(pix, q.HW - chunk * pix), e.x, e.y});
@@ -859,7 +861,9 @@ __global__ __launch_bounds__(256) void gn_finish_kernel(NormGeom q, int chunks, 
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = join(join(sh[0], sh[1]), join(sh[2], sh[3]));
+    s = sh[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) s = join(s, sh[w]);
     const uint32_t row = (q.n0 + n) * q.G + g;
     mean[row] = s.m;
     rstd[row] = 1.0f / sqrtf(s.M * q.inv_d + q.eps);
@@ -1028,25 +1032,28 @@ __global__ __launch_bounds__(256) void gn_dx_last_kernel(NormGeom q, LastTile t,
 }
 
 // Column sums of the K rows of pa and pb: a workgroup takes 32 channels and the rows [k0, k1), 8 lanes per channel walk over
-// them, then add up in order.
+// them, then add up in order: lanes behind the first 256 only pass the barrier, so the bits do not depend on the launch.
 __device__ __forceinline__ void column_sums(uint32_t block, int k0, int k1, int C, const float* pa, const float* pb, float* outa, int beta_a,
                                             float* outb, int beta_b) {
-  __shared__ float sh[2][8][33];
+  constexpr int S = 8;
+  __shared__ float sh[2][S][33];
   const int li = threadIdx.x & 31, lk = threadIdx.x >> 5, c = block * 32 + li;
   float a = 0.0f, b = 0.0f;
-  if (c < C) {
+  if (c < C && lk < S) {
 #pragma unroll 4
-    for (int k = k0 + lk; k < k1; k += 8) {
+    for (int k = k0 + lk; k < k1; k += S) {
       a += pa[(uint32_t)k * C + c];
       b += pb[(uint32_t)k * C + c];
     }
   }
-  sh[0][lk][li] = a;
-  sh[1][lk][li] = b;
+  if (lk < S) {
+    sh[0][lk][li] = a;
+    sh[1][lk][li] = b;
+  }
   __syncthreads();
   if (lk == 0 && c < C) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) {
+    for (int k = 1; k < S; ++k) {
       a += sh[0][k][li];
       b += sh[1][k][li];
     }
@@ -1057,9 +1064,10 @@ __device__ __forceinline__ void column_sums(uint32_t block, int k0, int k1, int 
 
 // row (n, g): s1 and s2 from the sums of its channels and chunks.  Workgroups behind the rows form dbeta and dgamma from the
 // K rows of the same sums, in the launch that is there anyway.
-__global__ __launch_bounds__(256) void gn_finish_dx_kernel(NormGeom q, int chunks, const float* gamma, const float* pa, const float* pb,
+template <int T>
+__global__ __launch_bounds__(T) void gn_finish_dx_kernel(NormGeom q, int chunks, const float* gamma, const float* pa, const float* pb,
                                                            float2* s12, int K, float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta) {
-  __shared__ float sh[2][4];
+  __shared__ float sh[2][T / 64];
   const uint32_t rows = (uint32_t)q.nb * q.G;
   if (blockIdx.x >= rows) {
     column_sums(blockIdx.x - rows, 0, K, q.C, pa, pb, dbeta, beta_dbeta, dgamma, beta_dgamma);
@@ -1067,14 +1075,14 @@ __global__ __launch_bounds__(256) void gn_finish_dx_kernel(NormGeom q, int chunk
   }
   const uint32_t n = q.n0 + blockIdx.x / q.G, g = blockIdx.x % q.G;
   float a = 0.0f, b = 0.0f;
-  for (int j = threadIdx.x; j < chunks * q.Cg; j += 256) {
+  for (int j = threadIdx.x; j < chunks * q.Cg; j += T) {
     const int chunk = j / q.Cg, c = g * q.Cg + (j - chunk * q.Cg);
     const float ga = gamma ? gamma[c] : 1.0f;
     a += ga * pa[(n * chunks + chunk) * q.C + c];
     b += ga * pb[(n * chunks + chunk) * q.C + c];
   }
-  a = sum_all<256>(a, sh[0]);
-  b = sum_all<256>(b, sh[1]);
+  a = sum_all<T>(a, sh[0]);
+  b = sum_all<T>(b, sh[1]);
   if (threadIdx.x == 0) s12[n * q.G + g] = make_float2(a * q.inv_d, b * q.inv_d);
 }
 
@@ -1324,7 +1332,7 @@ static SplitPlan split_plan(const DeviceCtx* ctx, const NormGeom& q) {
   s.chunks = (q.HW + s.pix - 1) / s.pix;
   s.sum_blocks = q.last ? (unsigned)s.sum.slabs * s.chunks : (unsigned)q.C * s.chunks;
   s.out_blocks = q.last ? (unsigned)s.out.slabs * s.out.chunks : (unsigned)q.C * s.chunks;
-  const uint64_t most = (1u << 23) / std::max({s.sum_blocks, s.out_blocks, (unsigned)q.G});   // no grid reaches 2^32 threads
+  const uint64_t most = (1u << 21) / std::max({s.sum_blocks, s.out_blocks, (unsigned)q.G});   // no grid reaches 2^32 threads
   s.images = (int)std::max<uint64_t>(1, std::min<uint64_t>(q.N, most));
   return s;
 }
@@ -1369,7 +1377,8 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
         hipLaunchKernelGGL(four ? gn_stats_last_kernel<G4> : gn_stats_last_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, part);
       else
         hipLaunchKernelGGL(four ? gn_stats_first_kernel<G4> : gn_stats_first_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, part);
-      hipLaunchKernelGGL(gn_finish_kernel, dim3((unsigned)(q.nb * q.G)), dim3(256), 0, ctx->stream, q, s.chunks, s.pix, part, mean, rstd);
+      const bool wide = s.chunks * q.Cg > 256;
+      hipLaunchKernelGGL(wide ? gn_finish_kernel<1024> : gn_finish_kernel<256>, dim3((unsigned)(q.nb * q.G)), dim3(wide ? 1024 : 256), 0, ctx->stream, q, s.chunks, s.pix, part, mean, rstd);
       if (q.last)
         hipLaunchKernelGGL((codes ? gn_apply_last_kernel<G4, true> :
                                 four ? gn_apply_last_kernel<G4, false> :
@@ -1405,7 +1414,9 @@ static void bwd_split(DeviceCtx* ctx, NormGeom q, const SplitPlan& s, SRC x, con
                               gn_sums_first_kernel<GANY, SRC>),
                              dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
     if (!dx) continue;
-    hipLaunchKernelGGL(gn_finish_dx_kernel, dim3((unsigned)(q.nb * q.G + (K ? (q.C + 31) / 32 : 0))), dim3(256), 0, ctx->stream, q, s.chunks, gamma,
+    const bool wide = s.chunks * q.Cg > 256;
+    hipLaunchKernelGGL(wide ? gn_finish_dx_kernel<1024> : gn_finish_dx_kernel<256>, dim3((unsigned)(q.nb * q.G + (K ? (q.C + 31) / 32 : 0))),
+                       dim3(wide ? 1024 : 256), 0, ctx->stream, q, s.chunks, gamma,
                        pa, pb, s12, K, dgamma, beta_dgamma, dbeta, beta_dbeta);
     if (q.last)
       hipLaunchKernelGGL((four ? gn_dx_last_kernel<G4, SRC> :
