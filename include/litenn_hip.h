@@ -341,6 +341,15 @@ int lnn_group_norm_fwd_f32(int dev, const lnn_group_norm_desc* d, const float* x
 int lnn_group_norm_bwd_f32(int dev, const lnn_group_norm_desc* d, const float* x, const void* x8, const float* gamma,
                            const float* beta, const float* mean, const float* rstd, const float* dy,
                            float* dx, int beta_dx, float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta);
+/* Which kernels serve a problem on a device with `compute_units` compute units: the forward pass, or the backward pass from
+ * x or (kept) from its 8-bit copy.  Host arithmetic only: works without a device.  info (2 values, may be NULL) receives the
+ * lanes that a row has and the groups of four elements (LNN_NORM_PATH_GATHERED_ROW: pixels) of a lane; 0, 0 for
+ * LNN_NORM_PATH_SPLIT. */
+#define LNN_NORM_PATH_ROWS 0             /* HW = 1, at most 8192 channels to a group: several rows to a workgroup */
+#define LNN_NORM_PATH_ROW_IN_REGISTERS 1 /* channels first: a workgroup holds its row and reads it once */
+#define LNN_NORM_PATH_GATHERED_ROW 2     /* channels last, small: a workgroup holds its row, element by element */
+#define LNN_NORM_PATH_SPLIT 3            /* the rest: sums, rows' statistics and result in launches of their own */
+int lnn_group_norm_path(const lnn_group_norm_desc* d, int backward, int kept, int compute_units, int* path, int32_t* info);
 
 /* ---- activations kept in 8 bits between the forward and the backward pass.
  *      Every 32 elements that follow each other in memory share a power of two 2^e: with a the largest magnitude among

@@ -104,6 +104,7 @@ SIGNATURES = {
     'lnn_bias_act_bwd_f32': [_c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _c_f32, _ptr, _ptr, _c_int],
     'lnn_group_norm_fwd_f32': [_c_int, ctypes.POINTER(GroupNormDesc)] + [_ptr] * 7,
     'lnn_group_norm_bwd_f32': [_c_int, ctypes.POINTER(GroupNormDesc)] + [_ptr] * 8 + [_c_int, _ptr, _c_int, _ptr, _c_int],
+    'lnn_group_norm_path': [ctypes.POINTER(GroupNormDesc), _c_int, _c_int, _c_int, ctypes.POINTER(_c_int), _i32arr],
     'lnn_bytes8': [_c_u64, ctypes.POINTER(_c_u64)],
     'lnn_encode8_f32': [_c_int, _c_u64, _ptr, _ptr],
     'lnn_decode8_f32': [_c_int, _c_u64, _ptr, _ptr],
@@ -408,6 +409,18 @@ def group_norm_bwd(dev, desc, x, x8, gamma, beta, mean, rstd, dy, dx, dgamma, db
     """Gradients of group_norm_fwd; x or its 8-bit copy x8 is given, the other is None.  dx, dgamma, dbeta may be None."""
     check(lib.lnn_group_norm_bwd_f32(dev, ctypes.byref(desc), x, x8, gamma, beta, mean, rstd, dy, dx, int(beta_dx),
                                      dgamma, int(beta_dgamma), dbeta, int(beta_dbeta)))
+
+
+NORM_PATH_ROWS, NORM_PATH_ROW_IN_REGISTERS, NORM_PATH_GATHERED_ROW, NORM_PATH_SPLIT = range(4)
+
+
+def group_norm_path(desc, backward, kept, compute_units):
+    """(path, lanes of a row, items per lane): the kernels that serve a group norm on a device with that many compute units
+    (host arithmetic, needs no device)."""
+    path = _c_int(-1)
+    info = (ctypes.c_int32 * 2)()
+    check(lib.lnn_group_norm_path(ctypes.byref(desc), int(backward), int(kept), int(compute_units), ctypes.byref(path), info))
+    return path.value, info[0], info[1]
 
 
 def bytes8(n):

@@ -1125,30 +1125,100 @@ static int make_geom(const lnn_group_norm_desc* d, NormGeom* q) {
   return LNN_OK;
 }
 
-// How a row is dealt out to a workgroup's lanes; false where it does not fit `most` groups of four per lane.
-struct ResPlan {
-  Units un;
+// ---- which kernel runs ------------------------------------------------------------------------------------------------
+//
+// The variants that are built: lanes and groups of four per lane, for a gathered row pixels per lane.  Plans pick from these lists
+// and launches switch over them, so that no plan can name a kernel that does not exist.
+#define LNN_RES_BWD(X)                                                                                 \
+  X(64, 1) X(256, 1) X(256, 2) X(256, 3) X(256, 4)                                                     \
+  X(512, 3) X(512, 4) X(512, 5) X(512, 6) X(512, 7) X(512, 8) X(512, 10) X(512, 13)                    \
+  X(1024, 2) X(1024, 3) X(1024, 4) X(1024, 5) X(1024, 6) X(1024, 7) X(1024, 8)
+#define LNN_RES_FWD(X) LNN_RES_BWD(X) X(512, 16) X(1024, 10) X(1024, 13) X(1024, 16)
+#define LNN_ROWS(X) X(4, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(256, 4) X(256, 8)
+#define LNN_GATHER(X) X(256, 1) X(256, 4) X(256, 8) X(256, 16) X(1024, 4) X(1024, 8) X(1024, 16)
+
+struct Variant {
   int T, V;
 };
-// most: groups per lane at 1024 lanes; most512: the same at 512
-static bool res_plan(const DeviceCtx* ctx, const NormGeom& q, int most, int most512, ResPlan* p) {
+#define LNN_VARIANT(T, V) {T, V},
+static const Variant kResBwd[] = {LNN_RES_BWD(LNN_VARIANT)};
+static const Variant kResFwd[] = {LNN_RES_FWD(LNN_VARIANT)};
+static const Variant kRows[] = {LNN_ROWS(LNN_VARIANT)};
+static const Variant kGather[] = {LNN_GATHER(LNN_VARIANT)};
+#undef LNN_VARIANT
+
+struct NormPlan {
+  int path;    // LNN_NORM_PATH_*
+  int T, V;    // of the path's list; 0 for the split kernels
+  int pt;      // gathered rows: pixels that the lanes hold at a time
+  Units un;    // rows in registers
+};
+
+// A row in registers; most, most512: groups per lane at 1024 and at 512 lanes.
+template <int N>
+static bool res_plan(const Variant (&list)[N], int cus, const NormGeom& q, int most, int most512, NormPlan* p) {
   if (q.last) return false;
   // the shortest unit that holds a plane, or whole wavefronts
   p->un.ul = q.HW <= 4 ? 0 : q.HW <= 16 ? 2 : q.HW <= 64 ? 4 : 6;
   p->un.per = ((q.HW + 3) / 4 + (1 << p->un.ul) - 1) >> p->un.ul;
-  const uint64_t lanes = ((uint64_t)q.Cg * p->un.per) << p->un.ul;
-  p->un.total = q.Cg * p->un.per;
-  if (lanes > 1024u * most || p->un.total > 3500) return false;   // 3500: two sums per unit, gamma and beta in 64 KB of LDS
+  const uint64_t units = (uint64_t)q.Cg * p->un.per, lanes = units << p->un.ul;
+  if (lanes > 1024u * most || units > 3500) return false;   // 3500: two sums per unit, gamma and beta in 64 KB of LDS
+  p->un.total = (int)units;
   p->un.dper = make_fastdiv((uint32_t)p->un.per);
-  p->T = lanes <= 64 ? 64 : lanes <= 1024 ? 256 : lanes <= 512u * most512 ? 512 : 1024;
-  if (lanes > 1024 && q.N * q.G <= ctx->cus) p->T = 1024;   // fewer rows than compute units: more lanes to each
-  static const int sizes[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 13, 16};
-  for (int v : sizes)
-    if (lanes <= (uint64_t)p->T * v) {
-      p->V = v;
+  int T = lanes <= 64 ? 64 : lanes <= 1024 ? 256 : lanes <= 512u * most512 ? 512 : 1024;
+  if (lanes > 1024 && q.N * q.G <= cus) T = 1024;   // fewer rows than compute units: more lanes to each
+  for (const Variant& v : list)
+    if (v.T == T && lanes <= (uint64_t)v.T * v.V) {
+      p->T = v.T;
+      p->V = v.V;
       return true;
     }
   return false;
+}
+
+// kept: x is read from its 8-bit copy (backward)
+static NormPlan norm_plan(int cus, const NormGeom& q, bool backward, bool kept) {
+  NormPlan p = {};
+  if (q.HW == 1) {
+    for (const Variant& v : kRows)
+      if (q.Cg <= 4 * v.T * v.V) {
+        p.path = LNN_NORM_PATH_ROWS;
+        p.T = v.T;
+        p.V = v.V;
+        return p;
+      }
+  }
+  if (backward ? res_plan(kResBwd, cus, q, 8, q.HW % 4 != 0 ? 8 : kept ? 13 : 10, &p)
+               : res_plan(kResFwd, cus, q, q.HW % 4 == 0 ? 16 : 13, 16, &p)) {
+    p.path = LNN_NORM_PATH_ROW_IN_REGISTERS;
+    return p;
+  }
+  if (q.last && q.HW > 1 && q.Cg <= 256 && q.size <= 1u << 20) {
+    for (const Variant& v : kGather)
+      if ((int64_t)(v.T / q.Cg) * v.V >= q.HW) {
+        p.path = LNN_NORM_PATH_GATHERED_ROW;
+        p.T = v.T;
+        p.V = v.V;
+        p.pt = v.T / q.Cg;
+        return p;
+      }
+  }
+  p.path = LNN_NORM_PATH_SPLIT;
+  return p;
+}
+
+int group_norm_path(const lnn_group_norm_desc* d, int backward, int kept, int cus, int* path, int32_t* info) {
+  if (!path || cus < 1) return set_error(LNN_ERR_INVALID, "group_norm_path: null pointer or no compute units");
+  NormGeom q;
+  const int st = make_geom(d, &q);
+  if (st != LNN_OK) return st;
+  const NormPlan p = norm_plan(cus, q, backward != 0, kept != 0);
+  *path = p.path;
+  if (info) {
+    info[0] = p.T;
+    info[1] = p.V;
+  }
+  return LNN_OK;
 }
 
 constexpr uint32_t kMaxRows = 1u << 21;   // of one launch
@@ -1190,49 +1260,6 @@ static void bwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const fl
                            dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un, SrcF{x}, gamma,
                        beta, mean, rstd, dy, dx, beta_dx, part);
 }
-#define LNN_RES_CASE(T, V, F, ...) \
-  case T * 32 + V: F<T, V>(__VA_ARGS__); break;
-#define LNN_RES_CASES(p, F, ...)                                                                                   \
-  switch ((p).T * 32 + (p).V) {                                                                                    \
-    LNN_RES_CASE(64, 1, F, __VA_ARGS__)                                                                            \
-    LNN_RES_CASE(256, 1, F, __VA_ARGS__) LNN_RES_CASE(256, 2, F, __VA_ARGS__) LNN_RES_CASE(256, 3, F, __VA_ARGS__) \
-    LNN_RES_CASE(256, 4, F, __VA_ARGS__)                                                                           \
-    LNN_RES_CASE(512, 3, F, __VA_ARGS__) LNN_RES_CASE(512, 4, F, __VA_ARGS__) LNN_RES_CASE(512, 5, F, __VA_ARGS__) \
-    LNN_RES_CASE(512, 6, F, __VA_ARGS__) LNN_RES_CASE(512, 7, F, __VA_ARGS__) LNN_RES_CASE(512, 8, F, __VA_ARGS__) \
-    LNN_RES_CASE(512, 10, F, __VA_ARGS__) LNN_RES_CASE(512, 13, F, __VA_ARGS__)                                    \
-    LNN_RES_CASE(1024, 2, F, __VA_ARGS__) LNN_RES_CASE(1024, 3, F, __VA_ARGS__) LNN_RES_CASE(1024, 4, F, __VA_ARGS__) \
-    LNN_RES_CASE(1024, 5, F, __VA_ARGS__) LNN_RES_CASE(1024, 6, F, __VA_ARGS__) LNN_RES_CASE(1024, 7, F, __VA_ARGS__) \
-    LNN_RES_CASE(1024, 8, F, __VA_ARGS__)
-
-// Lanes per row (L) and groups of four per lane (V) of the kernels for rows of channels alone; L = 0 where a row is longer.
-struct RowPlan {
-  int L, V;
-};
-static RowPlan row_plan(const NormGeom& q) {
-  const int d = q.Cg;
-  if (d <= 16) return {4, 1};
-  if (d <= 64) return {16, 1};
-  if (d <= 128) return {32, 1};
-  if (d <= 256) return {64, 1};
-  if (d <= 512) return {64, 2};
-  if (d <= 1024) return {64, 4};
-  if (d <= 2048) return {256, 2};
-  if (d <= 4096) return {256, 4};
-  if (d <= 8192) return {256, 8};
-  return {0, 0};
-}
-#define LNN_ROW_CASES(p, F, ...)                                \
-  switch ((p).L * 16 + (p).V) {                                 \
-    case 4 * 16 + 1: F<4, 1>(__VA_ARGS__); break;               \
-    case 16 * 16 + 1: F<16, 1>(__VA_ARGS__); break;             \
-    case 32 * 16 + 1: F<32, 1>(__VA_ARGS__); break;             \
-    case 64 * 16 + 1: F<64, 1>(__VA_ARGS__); break;             \
-    case 64 * 16 + 2: F<64, 2>(__VA_ARGS__); break;             \
-    case 64 * 16 + 4: F<64, 4>(__VA_ARGS__); break;             \
-    case 256 * 16 + 2: F<256, 2>(__VA_ARGS__); break;           \
-    case 256 * 16 + 4: F<256, 4>(__VA_ARGS__); break;           \
-    default: F<256, 8>(__VA_ARGS__); break;                     \
-  }
 template <int L, int V>
 static void fwd_rows(DeviceCtx* ctx, const NormGeom& q, const float* x, const float* gamma, const float* beta, float* y, float* mean,
                      float* rstd, uint8_t* codes, uint8_t* bytes) {
@@ -1267,28 +1294,6 @@ static void bwd_rows(DeviceCtx* ctx, const NormGeom& q, int chunks, const float*
                        dy, dx, beta_dx, part);
 }
 
-// Lanes and pixels per lane of the kernels for small channels-last problems; T = 0 where they do not apply.
-struct GatherPlan {
-  int T, V, pt;
-};
-static GatherPlan gather_plan(const NormGeom& q) {
-  GatherPlan p = {0, 0, 0};
-  if (!q.last || q.HW == 1 || q.Cg > 256 || q.size > 1u << 20) return p;
-  for (int T : {256, 1024})
-    for (int V : {1, 4, 8, 16}) {
-      const int pt = T / q.Cg;
-      if (p.T == 0 && (int64_t)pt * V >= q.HW) p = {T, V, pt};
-    }
-  return p;
-}
-#define LNN_GATHER_CASE(T, V, F, ...) \
-  case T * 32 + V: F<T, V>(__VA_ARGS__); break;
-#define LNN_GATHER_CASES(p, F, ...)                                                                                                       \
-  switch ((p).T * 32 + (p).V) {                                                                                                           \
-    LNN_GATHER_CASE(256, 1, F, __VA_ARGS__) LNN_GATHER_CASE(256, 4, F, __VA_ARGS__) LNN_GATHER_CASE(256, 8, F, __VA_ARGS__)               \
-    LNN_GATHER_CASE(256, 16, F, __VA_ARGS__) LNN_GATHER_CASE(1024, 8, F, __VA_ARGS__) LNN_GATHER_CASE(1024, 16, F, __VA_ARGS__)           \
-    default: return set_error(LNN_ERR_INVALID, "group_norm: no kernel for this plan");                                                    \
-  }
 template <int T, int V>
 static void fwd_gather(DeviceCtx* ctx, const NormGeom& q, int pt, const float* x, const float* gamma, const float* beta, float* y, float* mean,
                        float* rstd) {
@@ -1343,26 +1348,28 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   int st = make_geom(d, &q);
   if (st != LNN_OK) return st;
   const uint64_t n = (uint64_t)q.N * q.C * q.HW;
+  const NormPlan p = norm_plan(ctx->cus, q, false, false);
   // blocks of 32 lie inside a plane (channels first), a pixel's channels (last) or a row (one pixel): written on the way
-  const GatherPlan gp = gather_plan(q);
-  const bool whole = !gp.T && (!q.last ? q.HW : q.HW == 1 ? q.Cg : q.C) % 32 == 0;
+  const bool whole = p.path != LNN_NORM_PATH_GATHERED_ROW && (!q.last ? q.HW : q.HW == 1 ? q.Cg : q.C) % 32 == 0;
   uint8_t* codes = x8 && whole ? static_cast<uint8_t*>(x8) : nullptr;
   uint8_t* bytes = codes ? codes + n : nullptr;
-  ResPlan p;
-  if (q.HW == 1 && row_plan(q).L) {
-    LNN_ROW_CASES(row_plan(q), fwd_rows, ctx, q, x, gamma, beta, y, mean, rstd, codes, bytes)
-  } else if (gp.T) {
-    LNN_GATHER_CASES(gp, fwd_gather, ctx, q, gp.pt, x, gamma, beta, y, mean, rstd)
-  } else if (res_plan(ctx, q, q.HW % 4 == 0 ? 16 : 13, 16, &p)) {
+  if (p.path == LNN_NORM_PATH_ROWS) {
+#define LNN_LAUNCH(L, V) \
+  case L * 32 + V: fwd_rows<L, V>(ctx, q, x, gamma, beta, y, mean, rstd, codes, bytes); break;
+    switch (p.T * 32 + p.V) { LNN_ROWS(LNN_LAUNCH) }
+#undef LNN_LAUNCH
+  } else if (p.path == LNN_NORM_PATH_GATHERED_ROW) {
+#define LNN_LAUNCH(T, V) \
+  case T * 32 + V: fwd_gather<T, V>(ctx, q, p.pt, x, gamma, beta, y, mean, rstd); break;
+    switch (p.T * 32 + p.V) { LNN_GATHER(LNN_LAUNCH) }
+#undef LNN_LAUNCH
+  } else if (p.path == LNN_NORM_PATH_ROW_IN_REGISTERS) {
+#define LNN_LAUNCH(T, V) \
+  case T * 32 + V: fwd_res<T, V>(ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes); break;
     for (; q.row0 < (uint32_t)(q.N * q.G); q.row0 += kMaxRows) {
-      LNN_RES_CASES(p, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
-        LNN_RES_CASE(512, 16, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
-        LNN_RES_CASE(1024, 10, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
-        LNN_RES_CASE(1024, 13, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
-        LNN_RES_CASE(1024, 16, fwd_res, ctx, q, p.un, x, gamma, beta, y, mean, rstd, codes, bytes)
-        default: return set_error(LNN_ERR_INVALID, "group_norm: no kernel for this plan");
-      }
+      switch (p.T * 32 + p.V) { LNN_RES_FWD(LNN_LAUNCH) }
     }
+#undef LNN_LAUNCH
   } else {
     const SplitPlan s = split_plan(ctx, q);
     const bool four = (q.last ? q.C : q.HW) % 4 == 0;   // no tensor of fewer than four elements comes here
@@ -1441,30 +1448,21 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   const bool params = dgamma || dbeta;
   const uint8_t* codes = static_cast<const uint8_t*>(x8);
   const uint8_t* bytes = x8 ? codes + blocks8((uint64_t)q.N * q.C * q.HW) * 32 : nullptr;
+  const NormPlan p = norm_plan(ctx->cus, q, true, x8 != nullptr);
+  const bool split = p.path == LNN_NORM_PATH_SPLIT;
   // K rows of channel sums, and room for the rows that many of them are first brought down to
-  enum { kRows, kRes, kGather, kSplit } path;
-  const GatherPlan gp = gather_plan(q);
-  ResPlan p;
   SplitPlan s;
-  uint64_t K;
-  if (q.HW == 1 && row_plan(q).L) {
-    path = kRows;
-    const int slots = 256 / row_plan(q).L;   // four rows or more per slot, about eight workgroups per compute unit
+  uint64_t K = q.N;
+  if (p.path == LNN_NORM_PATH_ROWS) {
+    const int slots = 256 / p.T;   // four rows or more per slot, about eight workgroups per compute unit
     K = std::min<uint64_t>(((uint64_t)q.N + 4 * slots - 1) / (4 * slots), ((uint64_t)8 * ctx->cus + q.G - 1) / q.G);
-  } else if (res_plan(ctx, q, 8, q.HW % 4 != 0 ? 8 : x8 ? 13 : 10, &p)) {
-    path = kRes;
-    K = q.N;
-  } else if (gp.T) {
-    path = kGather;
-    K = q.N;
-  } else {
-    path = kSplit;
+  } else if (split) {
     s = split_plan(ctx, q);
     K = (uint64_t)q.N * s.chunks;
   }
   const uint64_t per = std::max<uint64_t>(256, (K + 511) / 512), K2 = K > 512 ? (K + per - 1) / per : 0;
-  const uint64_t sums = (params || path == kSplit) ? K * q.C : 0;
-  st = ensure_workspace(ctx, (2 * sums + 2 * K2 * q.C + (path == kSplit ? 2 * (uint64_t)q.N * q.G : 0)) * 4 + 16);
+  const uint64_t sums = (params || split) ? K * q.C : 0;
+  st = ensure_workspace(ctx, (2 * sums + 2 * K2 * q.C + (split ? 2 * (uint64_t)q.N * q.G : 0)) * 4 + 16);
   if (st != LNN_OK) return st;
   float* pa = sums ? static_cast<float*>(ctx->ws) : nullptr;
   float* pb = pa + sums;
@@ -1472,17 +1470,24 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   float* qb = qa + K2 * q.C;
   float2* s12 = reinterpret_cast<float2*>(qb + K2 * q.C);   // an even number of floats behind the start
   // dgamma and dbeta in the launch that finishes the rows' sums, where there is one such launch
-  const bool with = params && path == kSplit && dx && K2 == 0 && s.images == q.N;
-  if (path == kRows) {
-    LNN_ROW_CASES(row_plan(q), bwd_rows, ctx, q, (int)K, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa)
-  } else if (path == kRes) {
+  const bool with = params && split && dx && K2 == 0 && s.images == q.N;
+  if (p.path == LNN_NORM_PATH_ROWS) {
+#define LNN_LAUNCH(L, V) \
+  case L * 32 + V: bwd_rows<L, V>(ctx, q, (int)K, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa); break;
+    switch (p.T * 32 + p.V) { LNN_ROWS(LNN_LAUNCH) }
+#undef LNN_LAUNCH
+  } else if (p.path == LNN_NORM_PATH_ROW_IN_REGISTERS) {
+#define LNN_LAUNCH(T, V) \
+  case T * 32 + V: bwd_res<T, V>(ctx, q, p.un, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa); break;
     for (; q.row0 < (uint32_t)(q.N * q.G); q.row0 += kMaxRows) {
-      LNN_RES_CASES(p, bwd_res, ctx, q, p.un, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa)
-        default: return set_error(LNN_ERR_INVALID, "group_norm: no kernel for this plan");
-      }
+      switch (p.T * 32 + p.V) { LNN_RES_BWD(LNN_LAUNCH) }
     }
-  } else if (path == kGather) {
-    LNN_GATHER_CASES(gp, bwd_gather, ctx, q, gp.pt, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa)
+#undef LNN_LAUNCH
+  } else if (p.path == LNN_NORM_PATH_GATHERED_ROW) {
+#define LNN_LAUNCH(T, V) \
+  case T * 32 + V: bwd_gather<T, V>(ctx, q, p.pt, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa); break;
+    switch (p.T * 32 + p.V) { LNN_GATHER(LNN_LAUNCH) }
+#undef LNN_LAUNCH
   } else if (x8) {
     bwd_split(ctx, q, s, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, with ? (int)K : 0, dgamma, beta_dgamma, dbeta,
               beta_dbeta);

@@ -26,6 +26,7 @@ int launch_random_normal(DeviceCtx*, float*, uint64_t, uint32_t, double, double)
 int launch_group_norm_fwd(DeviceCtx*, const lnn_group_norm_desc*, const float*, const float*, const float*, float*, float*, float*, void*);
 int launch_group_norm_bwd(DeviceCtx*, const lnn_group_norm_desc*, const float*, const void*, const float*, const float*, const float*,
                           const float*, const float*, float*, int, float*, int, float*, int);
+int group_norm_path(const lnn_group_norm_desc*, int, int, int, int*, int32_t*);
 int launch_encode8(DeviceCtx*, uint64_t, const float*, void*);
 int launch_decode8(DeviceCtx*, uint64_t, const void*, float*);
 int launch_wgrad8(DeviceCtx*, int, int, int, int, const void*, const float*, float*, int);
@@ -561,6 +562,10 @@ int lnn_group_norm_bwd_f32(int dev, const lnn_group_norm_desc* d, const float* x
   if (!mean || !rstd || !dy) return set_error(LNN_ERR_INVALID, "group_norm_bwd: null pointer");
   CTX(dev);
   return launch_group_norm_bwd(ctx, d, x, x8, gamma, beta, mean, rstd, dy, dx, beta_dx, dgamma, beta_dgamma, dbeta, beta_dbeta);
+}
+
+int lnn_group_norm_path(const lnn_group_norm_desc* d, int backward, int kept, int compute_units, int* path, int32_t* info) {
+  return group_norm_path(d, backward, kept, compute_units, path, info);
 }
 
 int lnn_bytes8(uint64_t n, uint64_t* bytes) {
