@@ -114,7 +114,8 @@ struct Src8 {
   __device__ __forceinline__ void load(uint32_t at, int cnt, uint32_t size, float* v) const {
     const uint32_t q = load_codes<MODE>(codes, at, cnt, size);
     const uint32_t b0 = cnt > 0 ? at >> 5 : 0u;
-    const float s0 = step_of(bytes[b0]);
+    // a lane without elements reads block 0, whose step may be infinite: 0 * inf is no 0
+    const float first = step_of(bytes[b0]), s0 = cnt > 0 ? first : 0.0f;
     if (MODE == G4) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = code_at(q, k) * s0;
