@@ -395,8 +395,16 @@ def bias_act_bwd(dev, N, O, HW, y, dy, act, slope, dpre, dbias, beta_bias):
     check(lib.lnn_bias_act_bwd_f32(dev, N, O, HW, y, dy, act, float(slope), dpre, dbias, beta_bias))
 
 
+def _fit_int32(who, *extents):
+    """ctypes keeps the low 32 bits of a larger number without a word: refuse it."""
+    for v in extents:
+        if not -1 << 31 <= v < 1 << 31:
+            raise HipException(ERR_UNSUPPORTED, f'{who}: extent {v} does not fit 32 bits')
+
+
 def group_norm_desc(N, C, HW, groups, channels_last=False, act=ACT_NONE, slope=0.0, eps=1e-5):
     """Group normalisation of [N][C][HW] (or [N][HW][C]) followed by act (ACT_NONE / ACT_LEAKY_RELU / ACT_SILU)."""
+    _fit_int32('group_norm', N, C, HW, groups)
     return GroupNormDesc(N, C, HW, groups, 1 if channels_last else 0, act, slope, eps)
 
 
@@ -440,6 +448,7 @@ def decode8(dev, n, src, dst):
 
 def gemm_wgrad8(dev, batch, rows, K, M, x8, dO, dW, beta=0):
     """dW[b] (+)= X[b]^T . dO[b] with X [batch][rows][K] in 8 bits, dO [batch][rows][M], dW [batch][K][M]."""
+    _fit_int32('gemm_wgrad8', batch, rows, K, M)
     check(lib.lnn_gemm_wgrad8_f32(dev, batch, rows, K, M, x8, dO, dW, int(beta)))
 
 

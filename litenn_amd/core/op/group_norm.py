@@ -19,6 +19,7 @@ def group_norm(input_t, groups, gamma_t=None, beta_t=None, eps=1e-5, activation=
      activation     None | 'leaky_relu' (x >= 0 ? x : alpha*x) | 'relu' | 'silu' (x / (1 + exp(-x)))
      keep8          hold input_t in 8 bits from here on, as nn.keep8(input_t) does, the copy written in the same pass.
                     input_t must not be a parameter or gradient.
+    Tensors of less than 2 GiB, at most 4194304 channels.
 
     Gradients of input, gamma and beta, each accumulated, are formed together in one pass over input and output
     gradient; the activation's slope is formed again from the input.
