@@ -26,6 +26,8 @@ def group_norm(input_t, groups, gamma_t=None, beta_t=None, eps=1e-5, activation=
     """
     if activation not in _ACTS:
         raise ValueError(f'unknown activation {activation!r}: {", ".join(repr(a) for a in _ACTS)} are known')
+    if groups != int(groups):
+        raise ValueError(f'groups must be a whole number: {groups}')
     op = nc.Cacheton.get(_GroupNormOp, input_t.shape, int(groups), bool(channels_last), float(eps), activation,
                          float(alpha) if activation == 'leaky_relu' else 0.0)
     for name, t in (('gamma', gamma_t), ('beta', beta_t)):

@@ -1,4 +1,5 @@
-"""Sizes that the library's 32-bit extents cannot hold are refused, not taken modulo 2^32."""
+"""Sizes that the library's 32-bit extents cannot hold are refused, not taken modulo 2^32; groups are whole numbers."""
+import numpy as np
 import pytest
 
 from litenn_amd.core.hip import api
@@ -33,3 +34,7 @@ def test_through_tensors(nn_backend):
             nn.group_norm(t, 1, channels_last=last)
         assert e.value.code == api.ERR_UNSUPPORTED
     assert not x_t._get_buffers()[0].has_ptr()
+    small_t = nn.Tensor_from_value(np.ones((2, 5), np.float32))
+    for groups in (2.5, 0.5, 1.0000001):
+        with pytest.raises(ValueError, match='groups'):
+            nn.group_norm(small_t, groups)
