@@ -121,6 +121,12 @@ def _values(case, seed):
 
 
 def prepare(case, seed):
+    s = _state(case, seed)
+    torch.cuda.synchronize()      # see _own: the library's stream does not wait for torch's
+    return s
+
+
+def _state(case, seed):
     s = dict(case, **_values(case, seed))
     k = case['kind']
     if k == 'keep8':
@@ -147,6 +153,10 @@ SLOPE = 0.1
 
 
 def _own(s):
+    """The calls on torch's memory.  The library queues its work on a stream of its own, and neither stream waits for the
+    other: the inputs have to be written before the call (prepare waits for that), and a program that reads the outputs
+    through torch, writes into the state or lets go of it waits for the device first (torch.cuda.synchronize(), or
+    api.synchronize(0) for the library's stream alone).  Passes behind each other are in order."""
     from litenn_amd.core.hip import api
     p = {k: v.data_ptr() for k, v in s.items() if isinstance(v, torch.Tensor)}
     k = s['kind']
