@@ -9,6 +9,7 @@
 // Statistics, sums and all arithmetic are fp32; the variance is taken around the mean, never as a difference of
 // squares.
 #include <algorithm>
+#include <type_traits>
 
 #include "keep8.hpp"
 
@@ -1223,75 +1224,80 @@ int group_norm_path(const lnn_group_norm_desc* d, int backward, int kept, int cu
 
 constexpr uint32_t kMaxRows = 1u << 21;   // of one launch
 
+static unsigned rows_of_launch(const NormGeom& q) { return std::min((uint32_t)(q.N * q.G) - q.row0, kMaxRows); }
+
+// Planes that are not whole groups of four take GANY, a tensor of fewer than four elements GTINY.  8-bit copies are written on
+// the way (codes) only where planes are whole blocks of 32.
 template <int T, int V>
 static void fwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const float* x, const float* gamma, const float* beta, float* y,
                     float* mean, float* rstd, uint8_t* codes, uint8_t* bytes) {
-  const unsigned rows = (unsigned)(q.N * q.G) - q.row0 < kMaxRows ? (unsigned)(q.N * q.G) - q.row0 : kMaxRows;
+  auto kernel = gn_fwd_res_kernel<T, V, GANY, false>;
   if (codes)
-    hipLaunchKernelGGL((gn_fwd_res_kernel<T, V, G4, true>), dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
-                       mean, rstd, codes, bytes);
-  else
-    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_fwd_res_kernel<T, V, G4, false> :
-                            q.size >= 4 ? gn_fwd_res_kernel<T, V, GANY, false> :
-                            gn_fwd_res_kernel<T, V, T == 64 ? GTINY :
-                            GANY, false>),
-                           dim3(rows), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y,
-                       mean, rstd, codes, bytes);
+    kernel = gn_fwd_res_kernel<T, V, G4, true>;
+  else if (q.HW % 4 == 0)
+    kernel = gn_fwd_res_kernel<T, V, G4, false>;
+  if constexpr (T == 64) {
+    if (q.size < 4) kernel = gn_fwd_res_kernel<T, V, GTINY, false>;
+  }
+  hipLaunchKernelGGL(kernel, dim3(rows_of_launch(q)), dim3(T), (unsigned)q.Cg * 8, ctx->stream, q, un, x, gamma, beta, y, mean, rstd, codes,
+                     bytes);
+}
+template <int T, int V, class SRC>
+static void bwd_res_from(DeviceCtx* ctx, const NormGeom& q, const Units& un, SRC x, const float* gamma, const float* beta, const float* mean,
+                         const float* rstd, const float* dy, float* dx, int beta_dx, float* part) {
+  // groups of four lie in one block of a copy where planes are whole groups
+  using Hold = std::conditional_t<std::is_same_v<SRC, Src8>, Hold8, HoldF>;
+  auto kernel = gn_bwd_res_kernel<T, V, GANY, SRC, HoldF>;
+  if (q.HW % 4 == 0) kernel = gn_bwd_res_kernel<T, V, G4, SRC, Hold>;
+  if constexpr (T == 64) {
+    if (q.size < 4) kernel = gn_bwd_res_kernel<T, V, GTINY, SRC, HoldF>;
+  }
+  hipLaunchKernelGGL(kernel, dim3(rows_of_launch(q)), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un, x, gamma, beta, mean, rstd,
+                     dy, dx, beta_dx, part);
 }
 template <int T, int V>
 static void bwd_res(DeviceCtx* ctx, const NormGeom& q, const Units& un, const float* x, const uint8_t* codes, const uint8_t* bytes,
                     const float* gamma, const float* beta, const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx,
                     float* part) {
-  const unsigned rows = (unsigned)(q.N * q.G) - q.row0 < kMaxRows ? (unsigned)(q.N * q.G) - q.row0 : kMaxRows;
-  if (codes && q.HW % 4 == 0)
-    hipLaunchKernelGGL((gn_bwd_res_kernel<T, V, G4, Src8, Hold8>), dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
-                       Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
-  else if (codes)
-    hipLaunchKernelGGL((q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, Src8, HoldF> :
-                            gn_bwd_res_kernel<T, V, T == 64 ? GTINY :
-                            GANY, Src8, HoldF>),
-                           dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un,
-                       Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
+  if (codes)
+    bwd_res_from<T, V>(ctx, q, un, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((q.HW % 4 == 0 ? gn_bwd_res_kernel<T, V, G4, SrcF, HoldF> :
-                            q.size >= 4 ? gn_bwd_res_kernel<T, V, GANY, SrcF, HoldF> :
-                            gn_bwd_res_kernel<T, V, T == 64 ? GTINY :
-                            GANY, SrcF, HoldF>),
-                           dim3(rows), dim3(T), (unsigned)(un.total + q.Cg) * 8, ctx->stream, q, un, SrcF{x}, gamma,
-                       beta, mean, rstd, dy, dx, beta_dx, part);
+    bwd_res_from<T, V>(ctx, q, un, SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
 }
+
 template <int L, int V>
 static void fwd_rows(DeviceCtx* ctx, const NormGeom& q, const float* x, const float* gamma, const float* beta, float* y, float* mean,
                      float* rstd, uint8_t* codes, uint8_t* bytes) {
-  const unsigned blocks = ((unsigned)(q.N * q.G) + 256 / L - 1) / (256 / L);   // a row has at least D / 4 lanes: below 2^24
+  auto kernel = gn_fwd_rows_kernel<L, V, GANY, false>;
   if (codes)
-    hipLaunchKernelGGL((gn_fwd_rows_kernel<L, V, G4, true>), dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
-  else
-    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_fwd_rows_kernel<L, V, G4, false> :
-                            q.C >= 4 ? gn_fwd_rows_kernel<L, V, GANY, false> :
-                            gn_fwd_rows_kernel<L, V, L == 4 ? GTINY :
-                            GANY, false>),
-                           dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
+    kernel = gn_fwd_rows_kernel<L, V, G4, true>;
+  else if (q.Cg % 4 == 0)
+    kernel = gn_fwd_rows_kernel<L, V, G4, false>;
+  if constexpr (L == 4) {
+    if (q.C < 4) kernel = gn_fwd_rows_kernel<L, V, GTINY, false>;
+  }
+  const unsigned blocks = ((unsigned)(q.N * q.G) + 256 / L - 1) / (256 / L);   // a row has at least D / 4 lanes: below 2^24
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, ctx->stream, q, x, gamma, beta, y, mean, rstd, codes, bytes);
+}
+template <int L, int V, class SRC>
+static void bwd_rows_from(DeviceCtx* ctx, const NormGeom& q, int chunks, SRC x, const float* gamma, const float* beta, const float* mean,
+                          const float* rstd, const float* dy, float* dx, int beta_dx, float* part) {
+  auto kernel = gn_bwd_rows_kernel<L, V, GANY, SRC>;
+  if (q.Cg % 4 == 0) kernel = gn_bwd_rows_kernel<L, V, G4, SRC>;
+  if constexpr (L == 4) {
+    if (q.C < 4) kernel = gn_bwd_rows_kernel<L, V, GTINY, SRC>;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)chunks * q.G), dim3(256), 0, ctx->stream, q, chunks, x, gamma, beta, mean, rstd, dy, dx, beta_dx,
+                     part);
 }
 template <int L, int V>
 static void bwd_rows(DeviceCtx* ctx, const NormGeom& q, int chunks, const float* x, const uint8_t* codes, const uint8_t* bytes,
                      const float* gamma, const float* beta, const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx,
                      float* part) {
-  const unsigned blocks = (unsigned)chunks * q.G;
   if (codes)
-    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, Src8> :
-                            q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, Src8> :
-                            gn_bwd_rows_kernel<L, V, L == 4 ? GTINY :
-                            GANY, Src8>),
-                           dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, Src8{codes, bytes}, gamma, beta,
-                       mean, rstd, dy, dx, beta_dx, part);
+    bwd_rows_from<L, V>(ctx, q, chunks, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((q.Cg % 4 == 0 ? gn_bwd_rows_kernel<L, V, G4, SrcF> :
-                            q.C >= 4 ? gn_bwd_rows_kernel<L, V, GANY, SrcF> :
-                            gn_bwd_rows_kernel<L, V, L == 4 ? GTINY :
-                            GANY, SrcF>),
-                           dim3(blocks), dim3(256), 0, ctx->stream, q, chunks, SrcF{x}, gamma, beta, mean, rstd,
-                       dy, dx, beta_dx, part);
+    bwd_rows_from<L, V>(ctx, q, chunks, SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, part);
 }
 
 template <int T, int V>
@@ -1302,12 +1308,13 @@ static void fwd_gather(DeviceCtx* ctx, const NormGeom& q, int pt, const float* x
 template <int T, int V>
 static void bwd_gather(DeviceCtx* ctx, const NormGeom& q, int pt, const float* x, const uint8_t* codes, const uint8_t* bytes, const float* gamma,
                        const float* beta, const float* mean, const float* rstd, const float* dy, float* dx, int beta_dx, float* part) {
+  const dim3 grid((unsigned)(q.N * q.G)), block(T);
   if (codes)
-    hipLaunchKernelGGL((gn_bwd_gather_kernel<T, V, Src8>), dim3((unsigned)(q.N * q.G)), dim3(T), 0, ctx->stream, q, pt, Src8{codes, bytes}, gamma,
-                       beta, mean, rstd, dy, dx, beta_dx, part);
+    hipLaunchKernelGGL((gn_bwd_gather_kernel<T, V, Src8>), grid, block, 0, ctx->stream, q, pt, Src8{codes, bytes}, gamma, beta, mean, rstd, dy,
+                       dx, beta_dx, part);
   else
-    hipLaunchKernelGGL((gn_bwd_gather_kernel<T, V, SrcF>), dim3((unsigned)(q.N * q.G)), dim3(T), 0, ctx->stream, q, pt, SrcF{x}, gamma, beta,
-                       mean, rstd, dy, dx, beta_dx, part);
+    hipLaunchKernelGGL((gn_bwd_gather_kernel<T, V, SrcF>), grid, block, 0, ctx->stream, q, pt, SrcF{x}, gamma, beta, mean, rstd, dy, dx,
+                       beta_dx, part);
 }
 
 // The tile of the channels-last kernels, and the chunks of either layout.
@@ -1342,6 +1349,39 @@ static SplitPlan split_plan(const DeviceCtx* ctx, const NormGeom& q) {
   return s;
 }
 
+static bool whole_fours(const NormGeom& q) { return (q.last ? q.C : q.HW) % 4 == 0; }
+// The rows' sums are finished by 1024 lanes where a row has more channel-chunks than one walk of 256 lanes
+static bool wide_finish(const NormGeom& q, const SplitPlan& s) { return s.chunks * q.Cg > 256; }
+static unsigned split_blocks(const NormGeom& q, unsigned per_image) { return q.last ? q.nb * per_image : (q.nb * per_image + 3) / 4; }
+
+// No tensor of fewer than four elements comes here.
+static void fwd_split(DeviceCtx* ctx, NormGeom q, const SplitPlan& s, const float* x, const float* gamma, const float* beta, float* mean,
+                      float* rstd, float* y, uint8_t* codes, uint8_t* bytes, float2* part) {
+  const bool four = whole_fours(q), wide = wide_finish(q, s);
+  auto finish = wide ? gn_finish_kernel<1024> : gn_finish_kernel<256>;
+  for (; q.n0 < q.N; q.n0 += s.images) {
+    q.nb = std::min(q.N - q.n0, s.images);
+    const dim3 sums(split_blocks(q, s.sum_blocks)), results(split_blocks(q, s.out_blocks)), rows((unsigned)(q.nb * q.G)), block(256);
+    if (q.last) {
+      auto stats = four ? gn_stats_last_kernel<G4> : gn_stats_last_kernel<GANY>;
+      hipLaunchKernelGGL(stats, sums, block, 0, ctx->stream, q, s.sum, x, part);
+    } else {
+      auto stats = four ? gn_stats_first_kernel<G4> : gn_stats_first_kernel<GANY>;
+      hipLaunchKernelGGL(stats, sums, block, 0, ctx->stream, q, s.chunks, x, part);
+    }
+    hipLaunchKernelGGL(finish, rows, dim3(wide ? 1024 : 256), 0, ctx->stream, q, s.chunks, s.pix, part, mean, rstd);
+    if (q.last) {
+      auto apply = four ? gn_apply_last_kernel<G4, false> : gn_apply_last_kernel<GANY, false>;
+      if (codes) apply = gn_apply_last_kernel<G4, true>;
+      hipLaunchKernelGGL(apply, results, block, 0, ctx->stream, q, s.out, x, gamma, beta, mean, rstd, y, codes, bytes);
+    } else {
+      auto apply = four ? gn_apply_first_kernel<G4, false> : gn_apply_first_kernel<GANY, false>;
+      if (codes) apply = gn_apply_first_kernel<G4, true>;
+      hipLaunchKernelGGL(apply, results, block, 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, y, codes, bytes);
+    }
+  }
+}
+
 int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const float* x, const float* gamma, const float* beta,
                           float* y, float* mean, float* rstd, void* x8) {
   NormGeom q;
@@ -1372,69 +1412,48 @@ int launch_group_norm_fwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
 #undef LNN_LAUNCH
   } else {
     const SplitPlan s = split_plan(ctx, q);
-    const bool four = (q.last ? q.C : q.HW) % 4 == 0;   // no tensor of fewer than four elements comes here
     st = ensure_workspace(ctx, (uint64_t)s.images * s.chunks * q.C * 8);
     if (st != LNN_OK) return st;
-    float2* part = static_cast<float2*>(ctx->ws);
-    for (; q.n0 < q.N; q.n0 += s.images) {
-      q.nb = q.N - q.n0 < s.images ? q.N - q.n0 : s.images;
-      const unsigned blocks = q.last ? q.nb * s.sum_blocks : (q.nb * s.sum_blocks + 3) / 4;
-      const unsigned oblocks = q.last ? q.nb * s.out_blocks : (q.nb * s.out_blocks + 3) / 4;
-      if (q.last)
-        hipLaunchKernelGGL(four ? gn_stats_last_kernel<G4> : gn_stats_last_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, part);
-      else
-        hipLaunchKernelGGL(four ? gn_stats_first_kernel<G4> : gn_stats_first_kernel<GANY>, dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, part);
-      const bool wide = s.chunks * q.Cg > 256;
-      hipLaunchKernelGGL(wide ? gn_finish_kernel<1024> : gn_finish_kernel<256>, dim3((unsigned)(q.nb * q.G)), dim3(wide ? 1024 : 256), 0, ctx->stream, q, s.chunks, s.pix, part, mean, rstd);
-      if (q.last)
-        hipLaunchKernelGGL((codes ? gn_apply_last_kernel<G4, true> :
-                                four ? gn_apply_last_kernel<G4, false> :
-                                gn_apply_last_kernel<GANY, false>),
-                               dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x,
-                           gamma, beta, mean, rstd, y, codes, bytes);
-      else
-        hipLaunchKernelGGL((codes ? gn_apply_first_kernel<G4, true> :
-                                four ? gn_apply_first_kernel<G4, false> :
-                                gn_apply_first_kernel<GANY, false>),
-                               dim3(oblocks), dim3(256), 0, ctx->stream, q,
-                           s.chunks, x, gamma, beta, mean, rstd, y, codes, bytes);
-    }
+    fwd_split(ctx, q, s, x, gamma, beta, mean, rstd, y, codes, bytes, static_cast<float2*>(ctx->ws));
   }
   LNN_HIP(hipGetLastError());
   return x8 && !codes ? launch_encode8(ctx, n, x, x8) : LNN_OK;
 }
 
+// Where the channel sums go: K rows of them are added up in the launch that finishes the rows' sums (0: in one of its own)
+struct ChannelSums {
+  int K;
+  float* dgamma;
+  int beta_dgamma;
+  float* dbeta;
+  int beta_dbeta;
+};
 template <class SRC>
 static void bwd_split(DeviceCtx* ctx, NormGeom q, const SplitPlan& s, SRC x, const float* gamma, const float* beta, const float* mean,
-                      const float* rstd, const float* dy, float* dx, int beta_dx, float* pa, float* pb, float2* s12, int K, float* dgamma, int beta_dgamma, float* dbeta, int beta_dbeta) {
-  const bool four = (q.last ? q.C : q.HW) % 4 == 0;   // no tensor of fewer than four elements comes here
+                      const float* rstd, const float* dy, float* dx, int beta_dx, float* pa, float* pb, float2* s12, const ChannelSums& c) {
+  const bool four = whole_fours(q), wide = wide_finish(q, s);
+  auto finish = wide ? gn_finish_dx_kernel<1024> : gn_finish_dx_kernel<256>;
   for (; q.n0 < q.N; q.n0 += s.images) {
-    q.nb = q.N - q.n0 < s.images ? q.N - q.n0 : s.images;
-    const unsigned blocks = q.last ? q.nb * s.sum_blocks : (q.nb * s.sum_blocks + 3) / 4;
-    const unsigned oblocks = q.last ? q.nb * s.out_blocks : (q.nb * s.out_blocks + 3) / 4;
-    if (q.last)
-      hipLaunchKernelGGL((four ? gn_sums_last_kernel<G4, SRC> :
-                              gn_sums_last_kernel<GANY, SRC>),
-                             dim3(blocks), dim3(256), 0, ctx->stream, q, s.sum, x, gamma, beta, mean, rstd, dy, pa, pb);
-    else
-      hipLaunchKernelGGL((four ? gn_sums_first_kernel<G4, SRC> :
-                              gn_sums_first_kernel<GANY, SRC>),
-                             dim3(blocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
+    q.nb = std::min(q.N - q.n0, s.images);
+    const dim3 sums(split_blocks(q, s.sum_blocks)), results(split_blocks(q, s.out_blocks)), block(256);
+    if (q.last) {
+      auto kernel = four ? gn_sums_last_kernel<G4, SRC> : gn_sums_last_kernel<GANY, SRC>;
+      hipLaunchKernelGGL(kernel, sums, block, 0, ctx->stream, q, s.sum, x, gamma, beta, mean, rstd, dy, pa, pb);
+    } else {
+      auto kernel = four ? gn_sums_first_kernel<G4, SRC> : gn_sums_first_kernel<GANY, SRC>;
+      hipLaunchKernelGGL(kernel, sums, block, 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, pa, pb);
+    }
     if (!dx) continue;
-    const bool wide = s.chunks * q.Cg > 256;
-    hipLaunchKernelGGL(wide ? gn_finish_dx_kernel<1024> : gn_finish_dx_kernel<256>, dim3((unsigned)(q.nb * q.G + (K ? (q.C + 31) / 32 : 0))),
-                       dim3(wide ? 1024 : 256), 0, ctx->stream, q, s.chunks, gamma,
-                       pa, pb, s12, K, dgamma, beta_dgamma, dbeta, beta_dbeta);
-    if (q.last)
-      hipLaunchKernelGGL((four ? gn_dx_last_kernel<G4, SRC> :
-                              gn_dx_last_kernel<GANY, SRC>),
-                             dim3(oblocks), dim3(256), 0, ctx->stream, q, s.out, x, gamma, beta, mean, rstd, dy, s12, dx,
-                         beta_dx);
-    else
-      hipLaunchKernelGGL((four ? gn_dx_first_kernel<G4, SRC> :
-                              gn_dx_first_kernel<GANY, SRC>),
-                             dim3(oblocks), dim3(256), 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, s12,
-                         dx, beta_dx);
+    const dim3 rows((unsigned)(q.nb * q.G + (c.K ? (q.C + 31) / 32 : 0)));
+    hipLaunchKernelGGL(finish, rows, dim3(wide ? 1024 : 256), 0, ctx->stream, q, s.chunks, gamma, pa, pb, s12, c.K, c.dgamma, c.beta_dgamma,
+                       c.dbeta, c.beta_dbeta);
+    if (q.last) {
+      auto kernel = four ? gn_dx_last_kernel<G4, SRC> : gn_dx_last_kernel<GANY, SRC>;
+      hipLaunchKernelGGL(kernel, results, block, 0, ctx->stream, q, s.out, x, gamma, beta, mean, rstd, dy, s12, dx, beta_dx);
+    } else {
+      auto kernel = four ? gn_dx_first_kernel<G4, SRC> : gn_dx_first_kernel<GANY, SRC>;
+      hipLaunchKernelGGL(kernel, results, block, 0, ctx->stream, q, s.chunks, x, gamma, beta, mean, rstd, dy, s12, dx, beta_dx);
+    }
   }
 }
 
@@ -1488,16 +1507,18 @@ int launch_group_norm_bwd(DeviceCtx* ctx, const lnn_group_norm_desc* d, const fl
   case T * 32 + V: bwd_gather<T, V>(ctx, q, p.pt, x, codes, bytes, gamma, beta, mean, rstd, dy, dx, beta_dx, pa); break;
     switch (p.T * 32 + p.V) { LNN_GATHER(LNN_LAUNCH) }
 #undef LNN_LAUNCH
-  } else if (x8) {
-    bwd_split(ctx, q, s, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, with ? (int)K : 0, dgamma, beta_dgamma, dbeta,
-              beta_dbeta);
   } else {
-    bwd_split(ctx, q, s, SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, with ? (int)K : 0, dgamma, beta_dgamma, dbeta, beta_dbeta);
+    const ChannelSums c = {with ? (int)K : 0, dgamma, beta_dgamma, dbeta, beta_dbeta};
+    if (x8)
+      bwd_split(ctx, q, s, Src8{codes, bytes}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, c);
+    else
+      bwd_split(ctx, q, s, SrcF{x}, gamma, beta, mean, rstd, dy, dx, beta_dx, pa, pb, s12, c);
   }
   if (params && !with) {
     const unsigned cols = (unsigned)((q.C + 31) / 32);
     if (K2) {
-      hipLaunchKernelGGL(gn_params_kernel, dim3(cols, (unsigned)K2), dim3(256), 0, ctx->stream, (int)K, (int)per, q.C, pa, pb, qa, 0, qb, 0);
+      hipLaunchKernelGGL(gn_params_kernel, dim3(cols, (unsigned)K2), dim3(256), 0, ctx->stream, (int)K, (int)per, q.C, pa, pb, qa, 0, qb,
+                         0);
       pa = qa;
       pb = qb;
       K = K2;
