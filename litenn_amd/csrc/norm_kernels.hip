@@ -19,7 +19,7 @@ struct NormGeom {
   int N, C, HW, G, Cg, last, silu;
   int n0, nb;           // images of this launch
   float slope, eps;
-  float d, inv_d;       // D and 1 / D; means are divided by D: a row of equal values then has exactly their mean
+  float d, inv_d;       // D and 1 / D
   uint32_t D, size;     // elements of a row and of the tensor
   uint32_t row0;        // first row of this launch (a grid holds fewer than 2^32 threads)
 };
