@@ -90,6 +90,7 @@ typedef const __attribute__((address_space(1))) void* glb_void;
 struct W8 {
   int rows, K, M, batch;   // rows, batch: of this launch's part
   int b0, r0, all;         // its first batch item and row; rows of the whole operand
+  int k0, m0, ldk, ldm;    // its first columns of X and dO (K and M of them); columns of the whole operands
   int steps;               // of 32 rows
   int ipan, jpan;    // panels of 32 columns of X and dO, whole tiles
   uint32_t xblocks, xsize;   // blocks of the 8-bit copy; elements of X
@@ -109,7 +110,7 @@ __device__ __forceinline__ void w8_pack_x(const W8& w, int b, int r16, int pan0,
   float v[8][4];
 #pragma unroll
   for (int r = 0; r < 8; ++r)
-    x.load<MX>(((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * w.K + c, r0 + r < w.rows ? cnt : 0, w.xsize, v[r]);
+    x.load<MX>(((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * w.ldk + w.k0 + c, r0 + r < w.rows ? cnt : 0, w.xsize, v[r]);
   uint4* o = ap + (((uint64_t)b * 2 * w.steps + r16) * w.ipan + pan) * 64 + half * 32 + quad * 4;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -131,7 +132,7 @@ __device__ __forceinline__ void w8_pack_o(const W8& w, int b, int r16, int pan0,
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const bool in = c < w.M && r0 + r < w.rows;
-      const float d = dO[in ? ((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * w.M + c : 0u];
+      const float d = dO[in ? ((uint32_t)(w.b0 + b) * w.all + w.r0 + r0 + r) * w.ldm + w.m0 + c : 0u];
       v[j][r] = in ? d : 0.0f;
     }
   }
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(256) void w8_pack_kernel(W8 w, int xwgs, int owgs, 
 // workgroups of one XCD (every eighth) take a contiguous run of t, so that its L2 serves each fragment to several tiles.
 template <int PI, int PJ, int WI, int WJ>
 __global__ __launch_bounds__(64 * WI * WJ) void w8_kernel(W8 w, int ti, int tj, int splits, int per, const uint4* ap, const uint4* bp,
-                                                          float* out, int beta) {
+                                                          float* out, int ldo, uint64_t bstride, int beta) {
   constexpr int NI = PI * WI, NJ = PJ * WJ, NW = WI * WJ, FR = 2 * (NI + 3 * NJ), LPW = FR / NW;
   static_assert(FR % NW == 0, "whole fragments per wavefront");
   __shared__ uint4 lds[2][FR][64];
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void w8_kernel(W8 w, int ti, int tj, 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
-  float* o = out + (uint64_t)(splits > 1 ? t / tiles : b) * w.K * w.M;
+  float* o = out + (uint64_t)z * bstride;   // splits are one behind the other: z is b where there is one
 #pragma unroll
   for (int i = 0; i < PI; ++i)
 #pragma unroll
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void w8_kernel(W8 w, int ti, int tj, 
         for (int e = 0; e < 16; ++e) {
           const int k = k0 + 8 * (e >> 2) + (e & 3);
           if (k < w.K) {
-            float* at = o + (uint64_t)k * w.M + m;
+            float* at = o + (uint64_t)k * ldo + m;
             *at = beta ? *at + acc[i][j][e] : acc[i][j][e];
           }
         }
@@ -284,8 +285,10 @@ static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* 
   const int ti = (K + side - 1) / side, tj = (M + side - 1) / side;
   w.ipan = ti * side / 32;
   w.jpan = tj * side / 32;
-  // rows split until every compute unit has a tile (128: two), two steps at least to a split
-  const int64_t want = (int64_t)ctx->cus * (side == 256 ? 1 : 2) / tiles(side);
+  // rows split until every compute unit has a tile (128: two), two steps at least to a split; not in a run of columns, whose rows
+  // of dW lie apart, and which has a tile's worth of rows at most
+  const bool whole = K == w.ldk && M == w.ldm;
+  const int64_t want = whole ? (int64_t)ctx->cus * (side == 256 ? 1 : 2) / tiles(side) : 1;
   int splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, w.steps / 2));
   const int per = (w.steps + splits - 1) / splits;
   splits = (w.steps + per - 1) / per;
@@ -301,18 +304,20 @@ static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* 
   const int xwgs = (w.ipan + 15) / 16, owgs = (w.jpan + 15) / 16;
   const uint64_t pieces = (uint64_t)batch * 2 * w.steps * (xwgs + owgs);
   const dim3 pgrid((unsigned)std::min<uint64_t>(pieces, 1u << 20));
-  if (K % 4 == 0)   // rows of X are whole groups of four: no shifts
+  if (w.ldk % 4 == 0)   // rows of X are whole groups of four: no shifts
     hipLaunchKernelGGL((w8_pack_kernel<G4>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
   else
     hipLaunchKernelGGL((w8_pack_kernel<GANY>), pgrid, dim3(256), 0, ctx->stream, w, xwgs, owgs, codes, dO, ap, bp);
   const int64_t total = (int64_t)ti * tj * splits * batch;
   const dim3 grid((unsigned)((total + 7) / 8 * 8));
+  // partial results are dense; dW's rows are ldm apart
   float* out = splits > 1 ? pp : dW;
-  const int b0 = splits > 1 ? 0 : beta;
+  const int ldo = splits > 1 ? M : w.ldm, b0 = splits > 1 ? 0 : beta;
+  const uint64_t bstride = splits > 1 ? (uint64_t)K * M : (uint64_t)w.ldk * w.ldm;
   if (side == 256)
-    hipLaunchKernelGGL((w8_kernel<4, 2, 2, 4>), grid, dim3(512), 0, ctx->stream, w, ti, tj, splits, per, ap, bp, out, b0);
+    hipLaunchKernelGGL((w8_kernel<4, 2, 2, 4>), grid, dim3(512), 0, ctx->stream, w, ti, tj, splits, per, ap, bp, out, ldo, bstride, b0);
   else
-    hipLaunchKernelGGL((w8_kernel<2, 2, 2, 2>), grid, dim3(256), 0, ctx->stream, w, ti, tj, splits, per, ap, bp, out, b0);
+    hipLaunchKernelGGL((w8_kernel<2, 2, 2, 2>), grid, dim3(256), 0, ctx->stream, w, ti, tj, splits, per, ap, bp, out, ldo, bstride, b0);
   if (splits > 1)
     hipLaunchKernelGGL(w8_join_kernel, grid8(ctx, (uint64_t)K * M * batch), dim3(256), 0, ctx->stream, (uint32_t)K * M, splits, batch, pp, dW, beta);
   LNN_HIP(hipGetLastError());
@@ -321,15 +326,17 @@ static int wgrad8_part(DeviceCtx* ctx, W8 w, const uint8_t* codes, const float* 
 
 int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta) {
   W8 w = {};
-  w.K = K;
-  w.M = M;
   w.all = rows;
+  w.ldk = K;
+  w.ldm = M;
   w.xsize = (uint32_t)batch * rows * K;
   w.xblocks = (uint32_t)blocks8(w.xsize);
-  // The laid-out operands of one launch stay below a gigabyte: many small products go in groups, one product of very
-  // many rows in runs of rows, each added to the one before.
-  const uint64_t step = ((uint64_t)((K + 255) / 256) + 3 * (uint64_t)((M + 255) / 256)) * 16384;   // bytes of 32 rows, at most
-  const int64_t most = std::max<int64_t>(1, (int64_t)((1u << 30) / step));                         // steps of one launch
+  // The laid-out operands of one launch stay within a gigabyte: many small products go in groups, one product of very many rows
+  // in runs of rows, each added to the one before, and one of very many columns in runs of 2^22 of them (16384 tiles at least).
+  constexpr int kColumns = 1 << 22;
+  const int kc = std::min(K, kColumns), mc = std::min(M, kColumns);
+  const uint64_t step = ((uint64_t)((kc + 255) / 256) + 3 * (uint64_t)((mc + 255) / 256)) * 16384;   // bytes of 32 rows, at most
+  const int64_t most = std::max<int64_t>(1, (int64_t)((1u << 30) / step));                           // steps of one launch
   const int64_t steps = ((int64_t)rows + 31) / 32;
   const int group = (int)std::min<int64_t>(batch, std::max<int64_t>(1, most / steps));
   const int run = (int)std::min<int64_t>(rows, most * 32);
@@ -337,16 +344,21 @@ int launch_wgrad8(DeviceCtx* ctx, int batch, int rows, int K, int M, const void*
   uint64_t most_bytes = 0;
   for (int launch = 0; launch < 2; ++launch) {
     for (w.b0 = 0; w.b0 < batch; w.b0 += group)
-      for (w.r0 = 0;; w.r0 += run) {
-        w.batch = std::min(group, batch - w.b0);
-        w.rows = std::min(run, rows - w.r0);
-        w.steps = (w.rows + 31) / 32;
-        uint64_t need = 0;
-        int st = wgrad8_part(ctx, w, static_cast<const uint8_t*>(x8), dO, dW + (uint64_t)w.b0 * K * M, w.r0 > 0 ? 1 : beta, launch ? nullptr : &need);
-        if (st != LNN_OK) return st;
-        most_bytes = std::max(most_bytes, need);
-        if (run >= rows - w.r0) break;
-      }
+      for (w.k0 = 0; w.k0 < K; w.k0 += kc)
+        for (w.m0 = 0; w.m0 < M; w.m0 += mc)
+          for (w.r0 = 0;; w.r0 += run) {
+            w.batch = std::min(group, batch - w.b0);
+            w.K = std::min(kc, K - w.k0);
+            w.M = std::min(mc, M - w.m0);
+            w.rows = std::min(run, rows - w.r0);
+            w.steps = (w.rows + 31) / 32;
+            float* out = dW + ((uint64_t)w.b0 * K + w.k0) * M + w.m0;
+            uint64_t need = 0;
+            int st = wgrad8_part(ctx, w, static_cast<const uint8_t*>(x8), dO, out, w.r0 > 0 ? 1 : beta, launch ? nullptr : &need);
+            if (st != LNN_OK) return st;
+            most_bytes = std::max(most_bytes, need);
+            if (run >= rows - w.r0) break;
+          }
     if (!launch) {
       int st = ensure_workspace(ctx, most_bytes);
       if (st != LNN_OK) return st;
