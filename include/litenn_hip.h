@@ -363,7 +363,8 @@ int lnn_encode8_f32(int dev, uint64_t n, const float* src, void* dst);
 int lnn_decode8_f32(int dev, uint64_t n, const void* src, float* dst);
 /* Weight gradient of a dense layer from its kept input (matmul.py:64-67, whose first operand is then the 8-bit copy):
  *   dW[b][k][m] (+)= sum over the rows of X[b][row][k] * dO[b][row][m]
- * x8 is the copy of the whole dense X [batch][rows][K]; dO [batch][rows][M] and dW [batch][K][M] are dense fp32. */
+ * x8 is the copy of the whole dense X [batch][rows][K]; dO [batch][rows][M] and dW [batch][K][M] are dense fp32.  Products
+ * and sums are as exact as in fp32, but for values of dO below 2^-110, which are taken to 2^-126. */
 int lnn_gemm_wgrad8_f32(int dev, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta);
 
 #ifdef __cplusplus
