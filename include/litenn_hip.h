@@ -353,10 +353,11 @@ int lnn_group_norm_path(const lnn_group_norm_desc* d, int backward, int kept, in
 
 /* ---- activations kept in 8 bits between the forward and the backward pass.
  *      Every 32 elements that follow each other in memory share a power of two 2^e: with a the largest magnitude among
- *      them, e is the smallest whole number for which a * 2^-e < 127.5, kept within [-126, 121].  Codes are round-half-even(x * 2^-e) as int8, within +-127; an
- *      element reads back as code * 2^e, off by at most half of 2^e.  A copy of n elements is ceil(n / 32) * 32 codes (the
- *      last block padded with zeros) followed by ceil(n / 32) exponent bytes: e + 127, or 0 for a block of zeros, or 255
- *      for a block that holds an infinity or a NaN, all of which reads back as NaN. */
+ *      them, e is the smallest whole number for which a * 2^-e < 127.5, kept within [-126, 121].  Codes are
+ *      round-half-even(x * 2^-e) as int8, within +-127; an element reads back as code * 2^e, off by at most half of 2^e (by
+ *      less than 2^e where e is held at 121).  A copy of n elements is ceil(n / 32) * 32 codes (the last block padded with
+ *      zeros) followed by ceil(n / 32) exponent bytes: e + 127, or 0 for a block of zeros, or 255 for a block that holds
+ *      an infinity or a NaN, all of which reads back as NaN. */
 /* bytes of the copy of n elements (host arithmetic) */
 int lnn_bytes8(uint64_t n, uint64_t* bytes);
 int lnn_encode8_f32(int dev, uint64_t n, const float* src, void* dst);
@@ -364,7 +365,9 @@ int lnn_decode8_f32(int dev, uint64_t n, const void* src, float* dst);
 /* Weight gradient of a dense layer from its kept input (matmul.py:64-67, whose first operand is then the 8-bit copy):
  *   dW[b][k][m] (+)= sum over the rows of X[b][row][k] * dO[b][row][m]
  * x8 is the copy of the whole dense X [batch][rows][K]; dO [batch][rows][M] and dW [batch][K][M] are dense fp32.  Products
- * and sums are as exact as in fp32, but for values of dO below 2^-110, which are taken to 2^-126. */
+ * and sums are as exact as in fp32, but for values of dO below 2^-110, which are taken to 2^-126.
+ * Scratch: both operands laid out in bf16, 2 bytes per element of X and 6 per element of dO, rows and columns padded to whole
+ * tiles; about a gigabyte at most at a time.  It stays allocated and serves later calls (lnn_release_device lets go of it). */
 int lnn_gemm_wgrad8_f32(int dev, int batch, int rows, int K, int M, const void* x8, const float* dO, float* dW, int beta);
 
 #ifdef __cplusplus

@@ -6,7 +6,7 @@ def keep8(t):
     memory.
 
     The fp32 storage goes back to the pool; every 32 elements that follow each other in memory share a power of two and
-    are rounded to 7 bits and sign below it (off by at most 2^-7 of the largest of the 32).  Call it when the forward
+    are rounded to 7 bits and sign below it (off by at most 1 / 127 of the largest of the 32).  Call it when the forward
     pass has read t for the last time:
 
         h = conv1(x)

@@ -5,7 +5,8 @@
 //   q = x 2^-e rounded half to even, within +-127;  the value read back is q 2^e.
 // 2^-e is a normal fp32 number and the product with it is exact (or far below half a step), so a code has exactly one
 // right value, whichever kernel forms it, and every value read back is exactly a bf16 number (7 bits of magnitude).
-// The error is at most half a step, 2^(e-1) <= a 2^-7 (a whole step at the very top of the fp32 range, e = 121).
+// The error is at most half a step, 2^(e-1) <= a / 127.5 (2^-127 where e is held at -126; a whole step at the very top of the fp32
+// range, where it is held at 121).
 // Exponent byte: e + 127; 0 for a block of zeros; 255 for a block that holds an infinity or NaN.  Such a block's codes
 // are 0 and read back as NaN (0 * inf): a diverged activation stays visible.
 //
