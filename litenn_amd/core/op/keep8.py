@@ -3,7 +3,8 @@ import litenn_amd as nn
 
 def keep8(t):
     """Hold tensor t in 8 bits from here on: what a forward pass leaves for the backward pass takes a quarter of its
-    memory.
+    memory.  (A dense layer's weight gradient then needs scratch, one for all layers: 2 bytes per element of its input and
+    6 per element of its output gradient, at most about a gigabyte.)
 
     The fp32 storage goes back to the pool; every 32 elements that follow each other in memory share a power of two and
     are rounded to 7 bits and sign below it (off by at most 1 / 127 of the largest of the 32).  Call it when the forward

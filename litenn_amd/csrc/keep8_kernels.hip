@@ -76,9 +76,11 @@ int launch_decode8(DeviceCtx* ctx, uint64_t n, const void* src, float* dst) {
 // bf16 work, which is a fifth of the fp32 pipe's time.  The pipe takes bf16 inputs below 2^-126 for 0: of a dO below 2^-110
 // the parts under 2^-126 are lost.
 //
-// Measured: 8192 rows, 4096 x 4096: 0.69 ms = 1.2 PFLOP/s of bf16 work, 400 TFLOP/s of the product (the fp32 pipe's product of
-// decoded values: 2.0 ms), the main kernel alone 0.61 ms, 1.35 PFLOP/s: as a library's bf16 product of that size runs here.
-// Bound: the matrix pipe; the first pass, 435 MB of traffic in 77 us, is the rest.
+// Measured: 8192 rows, 4096 x 4096: 0.67-0.69 ms = 1.2 PFLOP/s of bf16 work, 400 TFLOP/s of the product (the fp32 pipe's product of
+// decoded values: 2.0 ms) in passes behind each other: main kernel 0.60, 1.4 PFLOP/s, as a library's bf16 product of that size
+// runs here.  In the first dozen passes after a pause it takes 0.62 to 0.85 ms, until the clock has settled.
+// Bound: the matrix pipe; the first pass, 444 MB of traffic in 75 us, is the rest.  Thin operands are laid out too: 16384 rows,
+// 4 x 4096: 198 us, four times what decoding and an fp32 product take.
 //
 // First pass: both operands are laid out as the matrix instruction reads them, 1 KB per fragment of 32 columns x 16 rows
 // (lane l holds column l % 32, rows 8 (l / 32) .. + 7), rows and columns padded with zeros to whole tiles.  The main kernel

@@ -578,7 +578,7 @@ __global__ __launch_bounds__(T) void gn_bwd_gather_kernel(NormGeom q, int pt, SR
 // second time from its end backwards, where what the first reading left in the 256 MB memory-side cache still is.
 // Taking the images in batches that fit that cache was slower (16 x 128 x 128 x 256 forward: 276 us in batches of 96 MB, 208 of
 // 160 MB, 166 in one): the cache saves less than each batch's three short launches cost.
-// 16 x 128 x 128 x 256 forward 160 us = 805 MB at 5.0 TB/s; 8 x 64 x 64 x 320 step from 8 bits 85 us.
+// 16 x 128 x 128 x 256 forward 162 us = 824 MB at 5.1 TB/s; 8 x 64 x 64 x 320 step from 8 bits 85 us.
 //
 // Means and sums of squared distances of two sets join as
 //   n = na + nb, d = mb - ma:  m = ma + d nb / n,  M = Ma + Mb + d^2 na nb / n
